@@ -61,7 +61,18 @@ enum {
   FMHA_I8_DEV_WAIT_O_FREE = 9,     /* MMA issuer waiting for the previous P.V to be drained */
   FMHA_I8_DEV_WAIT_DEBUG = 10,     /* a wait inside a debug kernel */
   FMHA_I8_DEV_WAIT_INFO = 11,      /* a role waiting for (or the scanner waiting to reuse) a unit's mask information */
-  FMHA_I8_DEV_WAIT_QUANT = 12      /* quantiser: a tile of the tensor */
+  FMHA_I8_DEV_WAIT_QUANT = 12,     /* quantiser: a tile of the tensor */
+  /* No wait, but an index in device memory that points outside its tensor (nothing was accessed there): words[2] = 0: lengths or offsets of
+   * sequence words[3]; 1: a page of sequence words[3]; 2: position or slot of token words[3]. */
+  FMHA_I8_DEV_BAD_INDEX = 13
+};
+
+/* Element types of the serving calls. */
+enum {
+  FMHA_I8_TYPE_I8 = 0,
+  FMHA_I8_TYPE_BF16 = 1,
+  FMHA_I8_TYPE_FP16 = 2,
+  FMHA_I8_TYPE_FP32 = 3
 };
 
 #define FMHA_I8_FLAG_USE_TCU 1u    /* mirrors the reference's use_tcu argument; must be set */
@@ -145,6 +156,62 @@ int fmha_i8_sm100_infer_host_slice(const float amax[5], const int desc[4],
                                    const void* host_q, const void* host_k, const void* host_v,
                                    const void* host_mask, void* host_o, int bh_begin, int bh_count,
                                    unsigned flags);
+
+/* ------------------------------------------------------------------------------------------------------------------------------
+ * Serving a causal language model: rotary positions and the int8 cache, attention over packed prompts, attention over the cache.  The
+ * reference has no counterpart.  Grouped heads: query heads h = 0 .. head_num - 1 read key head h / (head_num / head_num_kv).
+ *
+ * The scores are exact, the probabilities have 11 bits (fp16) instead of the 8 of the calls above, and the sums 24: the output is that of the
+ * softmax of the int8 inputs up to fp16 rounding of P, and the rounding to its own type.  Same bytes for the same call every time.
+ *
+ * desc6 = {batch_num, max_seq_q, max_seq_k, head_num, head_num_kv, head_dim}; head_dim 64 or 128, head_num a multiple of head_num_kv.
+ * Lengths live on the device: cu_seqlens_q (int32 [batch_num + 1], ascending from the first token of the first sequence to the
+ * end of the last one) says which tokens of q and o are whose.  A sequence may have no tokens, no keys or fewer keys than tokens: tokens that see
+ * no key give zeros.  Tokens behind the last sequence are left as they were.  max_seq_q and max_seq_k are upper bounds of the lengths, by
+ * which the work is divided; a longer sequence of keys is still computed in full, while tokens beyond max_seq_q may be left out (the device
+ * status words say so: FMHA_I8_DEV_BAD_INDEX).  Offsets that point outside the tensors are cut to them and reported the same way.
+ * causal: token i of n_q sees keys j <= i + n_k - n_q, so that the last token sees all; without FMHA_I8_FLAG_CAUSAL all tokens see all keys.
+ * q: int8, token t and head h at q + t * token stride + h * head_dim; o the same, int8 (requantised with amax[3] = o_amax), bf16 or fp16 (then
+ * amax[3] is not looked at, nor is amax[4]).  All tensors 16-byte aligned, token strides in elements, whole multiples of 16 bytes.
+ * flags: FMHA_I8_FLAG_USE_TCU, and FMHA_I8_FLAG_CAUSAL or not. */
+#define FMHA_I8_FLAG_CAUSAL 4u
+
+/* Attention over prompts packed one after the other.  k, v: int8 [total_k, head_num_kv, head_dim] with token strides; cu_seqlens_k like
+ * cu_seqlens_q (the same pointer for self-attention).  tokens[2] = {total_q, total_k}, the sizes of the buffers; strides[4] = those of q, k, v, o. */
+int fmha_i8_sm100_infer_packed(void* stream, const float amax[5], const int desc6[6], const void* q, const void* k, const void* v,
+                               const int* cu_seqlens_q, const int* cu_seqlens_k, void* o, int o_type, const long long tokens[2],
+                               const long long strides[4], unsigned flags);
+
+/* Attention of new tokens -- one per sequence, chunks, or both in one batch -- over a paged cache that already holds their own keys and
+ * values too.  k_cache, v_cache: int8 [num_pages, head_num_kv, page_size, head_dim], pages page_stride elements apart (head_num_kv *
+ * page_size * head_dim where they are dense; the same in both), page_size a power of two from 16 to 4096.  page_table: int32 [batch_num, table_width],
+ * rows table_stride entries apart: the pages of a sequence in order; seqlens_k: int32 [batch_num], keys of each sequence.  Entries behind a sequence's
+ * last page are not read.  cache[5] = {num_pages, page_size, page_stride, table_width, table_stride}; tokens = total_q; strides[2] = those of q, o. */
+int fmha_i8_sm100_infer_paged(void* stream, const float amax[5], const int desc6[6], const void* q, const void* k_cache, const void* v_cache,
+                              const int* page_table, const int* seqlens_k, const int* cu_seqlens_q, void* o, int o_type, long long tokens,
+                              const long long strides[2], const long long cache[5], unsigned flags);
+
+/* The table of rotations for positions 0 .. positions - 1: fp32 [2][positions][pairs][2], cosine and sine of position * inv_freq[i] times
+ * magnitude: a 32-bit value, and in the second plane what it leaves of the 64-bit one.  inv_freq: double [pairs] on the device; every way of
+ * stretching a model's context is a choice of inv_freq and magnitude. */
+int fmha_i8_sm100_rope_table(void* stream, const double* inv_freq, int pairs, long long positions, double magnitude, float* table);
+
+/* What stands between a projection and the attention: rotates q and k by the tokens' positions, quantises q, k and v symmetrically to
+ * int8 with the ranges amax[0..2], and stores k and v where the attention reads them.
+ *   q, k, v    in_type (bf16, fp16 or fp32), [tokens, heads, head_dim] with token strides (views of one fused projection will do)
+ *   rotation   of the first rot_dim elements of each head of q and k (0: none; a multiple of 16), in pairs of neighbours (interleaved) or of elements
+ *              i and i + rot_dim / 2: (x1 c - x2 s, x2 c + x1 s) with c, s from the table at the token's position (int32)
+ *   codes      clamp(floor(y * (127 / amax) + 1/2), -127, 127), those of 64-bit arithmetic exactly; not a number gives 0
+ *   q_out      int8 [tokens, head_num, head_dim]
+ *   slots      nullptr: k_out, v_out are int8 [tokens, head_num_kv, head_dim] (for fmha_i8_sm100_infer_packed).  Otherwise int64 [tokens]: they are caches as
+ *              in fmha_i8_sm100_infer_paged, and token t goes to page slot / page_size, place slot % page_size; a negative slot is not stored.  Two
+ *              tokens with the same slot leave a mixture of both there.
+ * dims[5] = {tokens, head_num, head_num_kv, head_dim, rot_dim}; strides[3] = those of q, k, v; positions_in_table; cache[3] = {num_pages, page_size,
+ * page_stride} (not looked at without slots).  A token whose position lies outside the table is left out, and a slot outside the cache is
+ * not stored; both are reported through the device status words.  No tokens: nothing happens. */
+int fmha_i8_sm100_rope_quantize_append(void* stream, const float amax[5], const long long dims[5], const void* q, const void* k, const void* v, int in_type,
+                                       const long long strides[3], const int* positions, const float* table, long long positions_in_table,
+                                       int interleaved, int8_t* q_out, int8_t* k_out, int8_t* v_out, const long long* slots, const long long cache[3]);
 
 /* Debug: how a call on this device would run, without running it: plan[0] = the kernel, plan[1] = CTAs that share the key tiles of a
  * query tile (1: none do), plan[2] = whole rounds of query tiles, one per SM, in front of the shared ones.  desc5 as in

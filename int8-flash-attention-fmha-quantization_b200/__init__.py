@@ -32,11 +32,13 @@ ERR_TOO_LARGE = -10
 ERR_DEVICE = -11
 ERR_BAD_FLAGS = -12
 FLAG_USE_TCU = 1
+FLAG_CAUSAL = 4      # serving calls: a token sees the keys up to its own
 FLAG_UINT8_P = 2     # P quantised as unsigned 8 bit, 255 levels (the reference README's planned variant)
 
 EXPORTS = (
     "fmha_i8_sm100_infer", "fmha_i8_sm100_infer_slice", "fmha_i8_sm100_infer_cross", "fmha_i8_sm100_calibrate_o_amax", "fmha_i8_sm100_infer_host",
     "fmha_i8_sm100_infer_host_slice", "fmha_i8_sm100_infer_policy",
+    "fmha_i8_sm100_infer_packed", "fmha_i8_sm100_infer_paged", "fmha_i8_sm100_rope_table", "fmha_i8_sm100_rope_quantize_append",
     "fmha_i8_sm100_debug_plan", "fmha_i8_sm100_debug_host_fetch", "fmha_i8_sm100_debug_qk", "fmha_i8_sm100_debug_pv", "fmha_i8_sm100_debug_simt", "fmha_i8_sm100_debug_simt_x", "fmha_i8_sm100_debug_wait_probe", "fmha_i8_sm100_debug_wait_loops",
     "fmha_i8_sm100_quantize_f32", "fmha_i8_sm100_quantize_f32_noalloc", "fmha_i8_sm100_debug_quantize_whole_chip", "fmha_i8_sm100_device_status", "fmha_i8_sm100_last_status", "fmha_i8_sm100_status_string",
     "fmha_i8_sm100_launch_count", "fmha_i8_sm100_version",
@@ -75,6 +77,21 @@ class AttnDataDescriptorX:
 
 
 @dataclass
+class AttnDataDescriptorGrouped:
+    """Shape of the serving calls: sequences of different lengths, head_num / head_num_kv query heads to a key head.  max_seq_q and
+    max_seq_k are upper bounds of the lengths, which live on the device."""
+    batch_num: int = 1
+    max_seq_q: int = 1
+    max_seq_k: int = 64
+    head_num: int = 4
+    head_num_kv: int = 4
+    head_dim: int = 64
+
+    def as_c(self):
+        return (ctypes.c_int * 6)(self.batch_num, self.max_seq_q, self.max_seq_k, self.head_num, self.head_num_kv, self.head_dim)
+
+
+@dataclass
 class FMHAParamI8:
     """Per-tensor symmetric quantisation ranges (real = int8 * amax / 127)."""
     q_amax: float = 0.0
@@ -106,6 +123,11 @@ def lib():
         L.fmha_i8_sm100_infer_policy.argtypes = [vp, fp, ip, vp, vp, vp, vp, vp, ctypes.c_int, ctypes.c_int, u, ctypes.c_int, vp]
         L.fmha_i8_sm100_infer_host.argtypes = [fp, ip, vp, vp, vp, vp, vp, u]
         L.fmha_i8_sm100_infer_host_slice.argtypes = [fp, ip, vp, vp, vp, vp, vp, ctypes.c_int, ctypes.c_int, u]
+        llp = ctypes.POINTER(ctypes.c_longlong)
+        L.fmha_i8_sm100_infer_packed.argtypes = [vp, fp, ip, vp, vp, vp, vp, vp, vp, ctypes.c_int, llp, llp, u]
+        L.fmha_i8_sm100_infer_paged.argtypes = [vp, fp, ip, vp, vp, vp, vp, vp, vp, vp, ctypes.c_int, ctypes.c_longlong, llp, llp, u]
+        L.fmha_i8_sm100_rope_table.argtypes = [vp, vp, ctypes.c_int, ctypes.c_longlong, ctypes.c_double, vp]
+        L.fmha_i8_sm100_rope_quantize_append.argtypes = [vp, fp, llp, vp, vp, vp, ctypes.c_int, llp, vp, vp, ctypes.c_longlong, ctypes.c_int, vp, vp, vp, vp, llp]
         L.fmha_i8_sm100_debug_plan.argtypes = [ip, ctypes.c_int, ip]
         L.fmha_i8_sm100_debug_host_fetch.argtypes = [ip, vp, vp, vp, vp]
         L.fmha_i8_sm100_debug_qk.argtypes = [vp, ip, vp, vp, vp]
@@ -222,6 +244,63 @@ def FMHAInferI8Policy(stream, fmha_param, attn_desc_x, q, k, v, padding_mask, o,
                                               FLAG_USE_TCU, policy, row_scratch)
     if check and st != OK:
         raise FmhaError(st, "FMHAInferI8Policy")
+    return st
+
+
+def FMHAInferI8Packed(stream, fmha_param, attn_desc, q, k, v, cu_seqlens_q, cu_seqlens_k, o, causal=True, check=True):
+    """Attention over prompts of different lengths, packed one after the other, with grouped heads.
+
+    q, o: [tokens, head_num, head_dim]; k, v: [key tokens, head_num_kv, head_dim]; views whose last two dimensions are contiguous will do (a
+    fused projection's).  q, k, v int8; o int8 (requantised with fmha_param.o_amax), bfloat16 or float16.  cu_seqlens_q, cu_seqlens_k: int32
+    [batch_num + 1] on the device, the tokens at which each sequence begins and the last one ends.  attn_desc is an
+    AttnDataDescriptorGrouped.  causal: the last token of a sequence sees all its keys, each before it one less.  Tokens without a key give
+    zeros, tokens behind the last sequence are left as they were.  Enqueues on `stream`, no synchronisation; tensors that do not fit
+    together raise ValueError."""
+    st = (_binding or _native()).infer_packed(stream, fmha_param, attn_desc, q, k, v, cu_seqlens_q, cu_seqlens_k, o,
+                                              FLAG_USE_TCU | (FLAG_CAUSAL if causal else 0))
+    if check and st != OK:
+        raise FmhaError(st, "FMHAInferI8Packed")
+    return st
+
+
+def FMHAInferI8Paged(stream, fmha_param, attn_desc, q, k_cache, v_cache, page_table, seqlens_k, cu_seqlens_q, o, causal=True, check=True):
+    """Attention of new tokens -- one per sequence, chunks of prompts, or both in one batch -- over a paged int8 cache that holds their own keys
+    and values already (rope_quantize_append puts them there).
+
+    k_cache, v_cache: int8 [pages, head_num_kv, page_size, head_dim], page_size a power of two from 16 to 4096; page_table: int32 [batch_num,
+    most pages], the pages of each sequence in order; seqlens_k: int32 [batch_num], keys of each sequence, the new ones included.  Both live on
+    the device, so that a captured call follows them.  Everything else as in FMHAInferI8Packed."""
+    st = (_binding or _native()).infer_paged(stream, fmha_param, attn_desc, q, k_cache, v_cache, page_table, seqlens_k, cu_seqlens_q, o,
+                                             FLAG_USE_TCU | (FLAG_CAUSAL if causal else 0))
+    if check and st != OK:
+        raise FmhaError(st, "FMHAInferI8Paged")
+    return st
+
+
+def rope_table(stream, inv_freq, table, magnitude=1.0, check=True):
+    """The rotations of all positions that a model uses, made once: table float32 [2, positions, 2 * pairs] from inv_freq float64 [pairs].
+
+    table[0, p, 2 i : 2 i + 2] = magnitude * (cos, sin)(p * inv_freq[i]), table[1] what these leave of the 64-bit values.  A base is
+    inv_freq[i] = base ** (-i / pairs); a longer context is other frequencies (all of them slower, the slow ones slower, another base), and a magnitude."""
+    st = (_binding or _native()).rope_table(stream, inv_freq, table, magnitude)
+    if check and st != OK:
+        raise FmhaError(st, "rope_table")
+    return st
+
+
+def rope_quantize_append(stream, fmha_param, q, k, v, positions, table, q_out, k_out, v_out, slots=None, interleaved=False, check=True):
+    """Rotates q and k by their tokens' positions, quantises q, k, v to int8 (ranges q_amax, k_amax, v_amax of fmha_param) and stores k and v
+    where the attention reads them, in one kernel.
+
+    q [tokens, head_num, head_dim], k, v [tokens, head_num_kv, head_dim]: bfloat16, float16 or float32, views whose last two dimensions are
+    contiguous will do.  positions: int32 [tokens].  table: of rope_table; its last dimension says how many elements of a head are rotated
+    (a multiple of 16; None: none), in pairs of neighbours (interleaved) or of elements half of that apart.  q_out: int8 [tokens, head_num, head_dim].
+    slots None: k_out, v_out int8 [tokens, head_num_kv, head_dim]; int64 [tokens]: they are caches [pages, head_num_kv, page_size, head_dim], and
+    token t goes to page slots[t] // page_size, place slots[t] % page_size, nowhere if negative.  The codes are floor(y * (127 / amax) + 1/2), at most +-127, of
+    64-bit arithmetic; not a number gives 0."""
+    st = (_binding or _native()).rope_append(stream, fmha_param, q, k, v, positions, table, q_out, k_out, v_out, slots, interleaved)
+    if check and st != OK:
+        raise FmhaError(st, "rope_quantize_append")
     return st
 
 

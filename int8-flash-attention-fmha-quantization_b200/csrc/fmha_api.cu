@@ -18,6 +18,7 @@
 #include "fmha_fwd64_sm100.cuh"
 #include "fmha_fwd_sm100.cuh"
 #include "fmha_host_sm100.cuh"
+#include "fmha_internal.h"
 #include "fmha_policy_sm100.cuh"
 #include "fmha_quant_sm100.cuh"
 
@@ -44,6 +45,7 @@ struct DeviceInfo {
   // One word of mapped, pinned host memory per device.  A kernel whose bounded wait runs out writes 1 to
   // it (besides the device status words), so the next host call can see the failure without synchronising.
   volatile unsigned* host_flag = nullptr;
+  unsigned* host_word = nullptr;             // the same word as the device sees it
   int sm_count = 0;
   int max_clusters[kClusterSizes] = {};      // clusters of 2, 4, 8 CTAs of the forward kernel that are resident at once
   bool quant_clusters_of_16 = false;         // one cluster of 16 CTAs of the quantiser can be resident
@@ -89,6 +91,7 @@ DeviceInfo* current_device(int* err) {
       return nullptr;
     }
     d.host_flag = static_cast<volatile unsigned*>(host_word);
+    d.host_word = static_cast<unsigned*>(dev_view);
     d.status = static_cast<unsigned*>(ptr);
   }
   return &d;
@@ -205,10 +208,8 @@ int set_kernel_attributes(DeviceInfo* d) {
 }
 
 // Driver entry points, fetched through the runtime so the library has no link-time libcuda dependency.
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-using ReplaceAddressFn = CUresult (*)(CUtensorMap*, void*);
+using fmha_host::EncodeTiledFn;
+using fmha_host::ReplaceAddressFn;
 using PointerAttributeFn = CUresult (*)(void*, CUpointer_attribute, CUdeviceptr);
 template <typename Fn> Fn driver_fn(const char* name) {
   void* f = nullptr;
@@ -706,6 +707,34 @@ int quantize_impl(void* stream, const float* x, long long n, int8_t* out, float*
 
 }  // namespace
 
+// What the other translation units of this library share with this one.
+namespace fmha_host {
+
+int finish(int status) { return ::finish(status); }
+
+int device_for_call(Device* out) {
+  int err = FMHA_I8_OK;
+  DeviceInfo* dev = current_device(&err);
+  if (!dev) return err;
+  cudaGetDevice(&out->index);
+  out->sm_count = dev->sm_count;
+  out->status = dev->status;
+  out->host_word = dev->host_word;
+  if (*dev->host_flag != 0u) {
+    *dev->host_flag = 0u;
+    return FMHA_I8_ERR_DEVICE;
+  }
+  return FMHA_I8_OK;
+}
+
+void count_launch() { g_launch_count.fetch_add(1, std::memory_order_relaxed); }
+
+EncodeTiledFn encode_tiled() { return encode_fn(); }
+
+ReplaceAddressFn replace_address() { return replace_address_fn(); }
+
+}  // namespace fmha_host
+
 extern "C" {
 
 int fmha_i8_sm100_infer(void* stream, const float amax[5], const int desc[4], const void* q, const void* k,
@@ -1050,7 +1079,7 @@ const char* fmha_i8_sm100_status_string(int status) {
     case FMHA_I8_ERR_BAD_SLICE: return "bh_begin/bh_count outside the batch*head range";
     case FMHA_I8_ERR_BAD_AMAX: return "amax values must be finite and positive";
     case FMHA_I8_ERR_TOO_LARGE: return "size beyond the maximum of this entry point";
-    case FMHA_I8_ERR_DEVICE: return "a device-side bounded wait ran out (see fmha_i8_sm100_device_status)";
+    case FMHA_I8_ERR_DEVICE: return "a device-side bounded wait ran out or an index pointed outside its tensor (see fmha_i8_sm100_device_status)";
     case FMHA_I8_ERR_BAD_FLAGS: return "an undefined flag bit is set";
     default: return "unknown status";
   }

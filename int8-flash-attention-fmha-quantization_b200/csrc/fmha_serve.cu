@@ -1,0 +1,340 @@
+// Host side of the serving calls (include/fmha_i8_c.h): rotary positions and the write into the cache, attention over packed prompts
+// and over the paged cache.  Argument checks, tensor maps, the choice of a kernel and the launch.
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+#include <mutex>
+#include <utility>
+
+#include "../../include/fmha_i8_c.h"
+#include "fmha_grouped_sm100.cuh"
+#include "fmha_internal.h"
+#include "fmha_rope_sm100.cuh"
+#include "fmha_rows_sm100.cuh"
+
+namespace {
+
+using namespace fmha;
+using fmha_host::Device;
+using fmha_host::finish;
+
+constexpr int kMaxDevices = 64;
+constexpr long long kMostRows = 0x7FFFFFFFLL;
+
+bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+bool power_of_two(long long n) { return n > 0 && (n & (n - 1)) == 0; }
+int log2_of(long long n) { int s = 0; while ((1LL << s) < n) ++s; return s; }
+int type_bytes(int type) { return type == FMHA_I8_TYPE_I8 ? 1 : type == FMHA_I8_TYPE_FP32 ? 4 : 2; }
+
+// What is asked of and set on a device once, before the first launch there.
+struct Once {
+  std::atomic<bool> done{false};
+  int clusters16_d64 = 0, clusters16_d128 = 0;        // clusters of 16 CTAs of the wide rows kernel that are resident at once
+};
+Once g_once[kMaxDevices];
+std::mutex g_once_mutex;
+
+template <typename... Params, typename... Args>
+int launch(void (*fn)(Params...), unsigned grid, unsigned block, size_t smem, cudaStream_t stream, unsigned cluster, Args&&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  cfg.attrs = attr;
+  attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  if (cluster != 0) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = cluster;
+    attr[cfg.numAttrs].val.clusterDim.y = 1;
+    attr[cfg.numAttrs++].val.clusterDim.z = 1;
+  }
+  fmha_host::count_launch();
+  if (cudaLaunchKernelEx(&cfg, fn, std::forward<Args>(args)...) == cudaSuccess) return FMHA_I8_OK;
+  cudaGetLastError();
+  return FMHA_I8_ERR_LAUNCH;
+}
+
+template <int D> using RowsCfg = rows::Cfg<D>;
+
+template <int D> int set_up_rows(int* clusters16) {
+  constexpr int W = RowsCfg<D>::kWarps, Wide = RowsCfg<D>::kWarpsWide;
+  auto set = [](const void* fn, size_t bytes) {
+    return cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) == cudaSuccess &&
+           cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess;
+  };
+  if (!set(reinterpret_cast<const void*>(&rows::rows_kernel<D, W>), sizeof(rows::Smem<D, W>)) ||
+      !set(reinterpret_cast<const void*>(&rows::rows_kernel<D, Wide>), sizeof(rows::Smem<D, Wide>))) {
+    cudaGetLastError();
+    return FMHA_I8_ERR_LAUNCH;
+  }
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 16;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(16);
+  cfg.blockDim = dim3(Wide * 32);
+  cfg.dynamicSmemBytes = sizeof(rows::Smem<D, Wide>);
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(clusters16, rows::rows_kernel<D, Wide>, &cfg) != cudaSuccess) *clusters16 = 0;
+  cudaGetLastError();
+  return FMHA_I8_OK;
+}
+
+int set_up(const Device& dev) {
+  Once& once = g_once[dev.index];
+  if (once.done.load(std::memory_order_acquire)) return FMHA_I8_OK;
+  std::lock_guard<std::mutex> lock(g_once_mutex);
+  if (once.done.load(std::memory_order_relaxed)) return FMHA_I8_OK;
+  int st;
+  if ((st = set_up_rows<64>(&once.clusters16_d64)) != FMHA_I8_OK) return st;
+  if ((st = set_up_rows<128>(&once.clusters16_d128)) != FMHA_I8_OK) return st;
+  once.done.store(true, std::memory_order_release);
+  return FMHA_I8_OK;
+}
+
+// Where the keys lie: [outer, heads, rows, D] with strides in bytes; box_rows rows at a time.
+struct KeyLayout {
+  long long outer, heads, rows, row_stride, head_stride, outer_stride;
+  int box_rows;
+};
+int key_map(CUtensorMap* map, const void* base, const KeyLayout& l, int D) {
+  auto fn = fmha_host::encode_tiled();
+  if (!fn) return FMHA_I8_ERR_DRIVER;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(l.rows), static_cast<cuuint64_t>(l.heads), static_cast<cuuint64_t>(l.outer)};
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(l.row_stride), static_cast<cuuint64_t>(l.head_stride), static_cast<cuuint64_t>(l.outer_stride)};
+  const cuuint32_t box[4] = {static_cast<cuuint32_t>(D), static_cast<cuuint32_t>(l.box_rows), 1u, 1u}, ones[4] = {1u, 1u, 1u, 1u};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? FMHA_I8_OK : FMHA_I8_ERR_DRIVER;
+}
+
+struct Call {
+  grouped::Params p{};
+  const void *k = nullptr, *v = nullptr;
+  KeyLayout lk{}, lv{};
+  int D = 0;
+  long long max_k = 0;
+};
+
+// Checks and parameters that packed and paged calls share.
+int fill_call(Call* c, const float amax[5], const int desc6[6], const void* q, const void* k, const void* v, const int* cu_q, void* o, int o_type, long long total_q,
+              long long q_stride, long long o_stride, unsigned flags) {
+  if (!(flags & FMHA_I8_FLAG_USE_TCU)) return FMHA_I8_ERR_NO_CUDA_CORE_PATH;
+  if (flags & ~(FMHA_I8_FLAG_USE_TCU | FMHA_I8_FLAG_CAUSAL)) return FMHA_I8_ERR_BAD_FLAGS;
+  const int B = desc6[0], max_q = desc6[1], max_k = desc6[2], H = desc6[3], Hkv = desc6[4], D = desc6[5];
+  if (B < 1 || max_q < 0 || max_k < 0 || H < 1 || Hkv < 1 || H % Hkv != 0 || (D != 64 && D != 128)) return FMHA_I8_ERR_BAD_SHAPE;
+  if (o_type != FMHA_I8_TYPE_I8 && o_type != FMHA_I8_TYPE_BF16 && o_type != FMHA_I8_TYPE_FP16) return FMHA_I8_ERR_BAD_SHAPE;
+  if (total_q < 0 || q_stride < static_cast<long long>(H) * D || o_stride < static_cast<long long>(H) * D) return FMHA_I8_ERR_BAD_SHAPE;
+  const int G = H / Hkv;
+  if (total_q * H > kMostRows || static_cast<long long>(max_q) * G > kMostRows - 256 || max_k > (1 << 30)) return FMHA_I8_ERR_TOO_LARGE;
+  if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(o, 16) || !aligned(cu_q, 4)) return FMHA_I8_ERR_MISALIGNED;
+  if (q_stride % 16 != 0 || o_stride * type_bytes(o_type) % 16 != 0) return FMHA_I8_ERR_MISALIGNED;
+  for (int i = 0; i < (o_type == FMHA_I8_TYPE_I8 ? 4 : 3); ++i)
+    if (!(amax[i] > 0.f) || !std::isfinite(amax[i])) return FMHA_I8_ERR_BAD_AMAX;
+  grouped::Params& p = c->p;
+  const double c2 = static_cast<double>(amax[0]) * amax[1] / (127.0 * 127.0) / std::sqrt(static_cast<double>(D)) * 1.4426950408889634;
+  // between factors at which all probabilities are 1 and at which only the largest counts (the scores are integers up to 2^21)
+  p.c2 = static_cast<float>(std::min(std::max(c2, 0x1p-100), 64.0));
+  p.out_scale = o_type == FMHA_I8_TYPE_I8 ? static_cast<float>(static_cast<double>(amax[2]) / amax[3]) : amax[2] / 127.f;
+  if (!std::isfinite(p.out_scale)) return FMHA_I8_ERR_BAD_AMAX;
+  p.q = static_cast<const int8_t*>(q);
+  p.o = o;
+  p.q_stride = q_stride;
+  p.o_stride = o_stride;
+  p.cu_q = cu_q;
+  p.B = B; p.H = H; p.Hkv = Hkv; p.G = G;
+  p.total_q = static_cast<int>(total_q);
+  p.max_q = max_q;
+  p.o_type = o_type;
+  p.causal = (flags & FMHA_I8_FLAG_CAUSAL) != 0u;
+  c->k = k;
+  c->v = v;
+  c->D = D;
+  c->max_k = max_k;
+  return FMHA_I8_OK;
+}
+
+template <int D> int launch_rows(cudaStream_t stream, const Device& dev, Call& c, const CUtensorMap& mk, const CUtensorMap& mv) {
+  grouped::Params& p = c.p;
+  constexpr int W = RowsCfg<D>::kWarps, Wide = RowsCfg<D>::kWarpsWide;
+  p.row_groups = static_cast<int>((static_cast<long long>(p.max_q) * p.G + rows::kRows - 1) / rows::kRows);
+  const long long units = static_cast<long long>(p.B) * p.Hkv * p.row_groups;
+  const long long n_tiles = (c.max_k + grouped::kTile - 1) / grouped::kTile;
+  if (units > kMostRows / rows::kMaxCluster) return FMHA_I8_ERR_TOO_LARGE;
+  const long long resident = 3LL * dev.sm_count;
+  int ctas = 1;
+  while (ctas < 8 && ((units * ctas < 2 * resident && n_tiles >= 4 * ctas * W) || (units * ctas * 2 <= resident && n_tiles >= 2 * ctas * W))) ctas *= 2;
+  const int clusters16 = D == 128 ? g_once[dev.index].clusters16_d128 : g_once[dev.index].clusters16_d64;
+  if (ctas == 8 && units <= clusters16 && n_tiles >= 32 * Wide)
+    return launch(rows::rows_kernel<D, Wide>, static_cast<unsigned>(units * 16), Wide * 32, sizeof(rows::Smem<D, Wide>), stream, 16u, mk, mv, p);
+  return launch(rows::rows_kernel<D, W>, static_cast<unsigned>(units * ctas), W * 32, sizeof(rows::Smem<D, W>), stream, static_cast<unsigned>(ctas), mk, mv, p);
+}
+
+int run_attention(void* stream, Call& c) {
+  Device dev;
+  int st;
+  if ((st = fmha_host::device_for_call(&dev)) != FMHA_I8_OK) return st;
+  if ((st = set_up(dev)) != FMHA_I8_OK) return st;
+  if (c.p.total_q == 0 || c.p.max_q == 0) return FMHA_I8_OK;
+  c.p.status = dev.status;
+  c.p.host_word = dev.host_word;
+  CUtensorMap mk, mv;
+  if ((st = key_map(&mk, c.k, c.lk, c.D)) != FMHA_I8_OK) return st;
+  if ((st = key_map(&mv, c.v, c.lv, c.D)) != FMHA_I8_OK) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return c.D == 128 ? launch_rows<128>(s, dev, c, mk, mv) : launch_rows<64>(s, dev, c, mk, mv);
+}
+
+int infer_packed_impl(void* stream, const float amax[5], const int desc6[6], const void* q, const void* k, const void* v, const int* cu_q, const int* cu_k, void* o,
+                      int o_type, const long long tokens[2], const long long strides[4], unsigned flags) {
+  if (!amax || !desc6 || !q || !k || !v || !cu_q || !cu_k || !o || !tokens || !strides) return FMHA_I8_ERR_NULL_POINTER;
+  Call c;
+  const int st = fill_call(&c, amax, desc6, q, k, v, cu_q, o, o_type, tokens[0], strides[0], strides[3], flags);
+  if (st != FMHA_I8_OK) return st;
+  const long long width = static_cast<long long>(c.p.Hkv) * c.D;
+  if (tokens[1] < 0 || strides[1] < width || strides[2] < width) return FMHA_I8_ERR_BAD_SHAPE;
+  if (tokens[1] > (1LL << 30)) return FMHA_I8_ERR_TOO_LARGE;
+  if (strides[1] % 16 != 0 || strides[2] % 16 != 0 || !aligned(cu_k, 4)) return FMHA_I8_ERR_MISALIGNED;
+  c.p.cu_k = cu_k;
+  c.p.total_k = static_cast<int>(tokens[1]);
+  c.p.num_pages = 1;
+  c.p.page_shift = 0;
+  c.p.box_shift = log2_of(grouped::kTile);
+  const long long rows = std::max(tokens[1], 1LL);
+  c.lk = KeyLayout{1, c.p.Hkv, rows, strides[1], c.D, strides[1] * rows, grouped::kTile};
+  c.lv = KeyLayout{1, c.p.Hkv, rows, strides[2], c.D, strides[2] * rows, grouped::kTile};
+  return run_attention(stream, c);
+}
+
+int infer_paged_impl(void* stream, const float amax[5], const int desc6[6], const void* q, const void* k, const void* v, const int* page_table, const int* lens_k,
+                     const int* cu_q, void* o, int o_type, long long tokens, const long long strides[2], const long long cache[5], unsigned flags) {
+  if (!amax || !desc6 || !q || !k || !v || !page_table || !lens_k || !cu_q || !o || !strides || !cache) return FMHA_I8_ERR_NULL_POINTER;
+  Call c;
+  const int st = fill_call(&c, amax, desc6, q, k, v, cu_q, o, o_type, tokens, strides[0], strides[1], flags);
+  if (st != FMHA_I8_OK) return st;
+  const long long pages = cache[0], page = cache[1], page_stride = cache[2], width = cache[3], table_stride = cache[4];
+  if (pages < 1 || !power_of_two(page) || page < 16 || page > 4096 || page_stride < c.p.Hkv * page * c.D || width < 1 || table_stride < width) return FMHA_I8_ERR_BAD_SHAPE;
+  if (pages > 0x7FFFFFFELL || width > ((1LL << 30) / page)) return FMHA_I8_ERR_TOO_LARGE;
+  if (page_stride % 16 != 0 || !aligned(page_table, 4) || !aligned(lens_k, 4)) return FMHA_I8_ERR_MISALIGNED;
+  c.p.lens_k = lens_k;
+  c.p.page_table = page_table;
+  c.p.table_stride = table_stride;
+  c.p.table_width = static_cast<int>(width);
+  c.p.page_shift = log2_of(page);
+  c.p.num_pages = static_cast<int>(pages);
+  c.p.box_shift = std::min(c.p.page_shift, log2_of(grouped::kTile));
+  c.lk = KeyLayout{pages, c.p.Hkv, page, c.D, page * c.D, page_stride, 1 << c.p.box_shift};
+  c.lv = c.lk;
+  c.max_k = std::min(c.max_k, width * page);
+  return run_attention(stream, c);
+}
+
+int rope_table_impl(void* stream, const double* inv_freq, int pairs, long long positions, double magnitude, float* table) {
+  if (!inv_freq || !table) return FMHA_I8_ERR_NULL_POINTER;
+  if (pairs < 1 || pairs > 64 || positions < 0) return FMHA_I8_ERR_BAD_SHAPE;
+  if (positions > 0x7FFFFFFFLL) return FMHA_I8_ERR_TOO_LARGE;
+  if (!std::isfinite(magnitude)) return FMHA_I8_ERR_BAD_AMAX;
+  if (!aligned(inv_freq, 8) || !aligned(table, 16)) return FMHA_I8_ERR_MISALIGNED;
+  Device dev;
+  const int st = fmha_host::device_for_call(&dev);
+  if (st != FMHA_I8_OK || positions == 0) return st;
+  const long long blocks = std::min((positions * pairs + 255) / 256, 32LL * dev.sm_count);
+  rope::rope_table_kernel<<<static_cast<unsigned>(blocks), 256, 0, static_cast<cudaStream_t>(stream)>>>(inv_freq, pairs, positions, magnitude, table);
+  fmha_host::count_launch();
+  return cudaGetLastError() == cudaSuccess ? FMHA_I8_OK : FMHA_I8_ERR_LAUNCH;
+}
+
+template <typename T> int launch_append(cudaStream_t stream, const rope::Params& p, int D, unsigned grid) {
+  return D == 128 ? launch(rope::append_kernel<128, T>, grid, rope::kThreads, 0, stream, 0u, p) : launch(rope::append_kernel<64, T>, grid, rope::kThreads, 0, stream, 0u, p);
+}
+
+int append_impl(void* stream, const float amax[5], const long long dims[5], const void* q, const void* k, const void* v, int in_type, const long long strides[3],
+                const int* positions, const float* table, long long in_table, int interleaved, int8_t* q_out, int8_t* k_out, int8_t* v_out, const long long* slots,
+                const long long cache[3]) {
+  if (!amax || !dims || !q || !k || !v || !strides || !positions || !q_out || !k_out || !v_out || (slots && !cache)) return FMHA_I8_ERR_NULL_POINTER;
+  const long long tokens = dims[0], H = dims[1], Hkv = dims[2], D = dims[3], rot = dims[4];
+  if (tokens < 0 || H < 1 || Hkv < 1 || (D != 64 && D != 128) || rot < 0 || rot > D || rot % 16 != 0) return FMHA_I8_ERR_BAD_SHAPE;
+  if (in_type != FMHA_I8_TYPE_BF16 && in_type != FMHA_I8_TYPE_FP16 && in_type != FMHA_I8_TYPE_FP32) return FMHA_I8_ERR_BAD_SHAPE;
+  if (rot > 0 && !table) return FMHA_I8_ERR_NULL_POINTER;
+  if (in_table < 0 || strides[0] < H * D || strides[1] < Hkv * D || strides[2] < Hkv * D) return FMHA_I8_ERR_BAD_SHAPE;
+  if (H > 65536 || Hkv > 65536 || tokens * (H + 2 * Hkv) > kMostRows || in_table > kMostRows) return FMHA_I8_ERR_TOO_LARGE;
+  for (int i = 0; i < 3; ++i)
+    if (!(amax[i] > 0.f) || !std::isfinite(amax[i]) || !std::isfinite(127.f / amax[i])) return FMHA_I8_ERR_BAD_AMAX;
+  const int bytes = type_bytes(in_type);
+  if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(table, 16) || !aligned(positions, 4) || !aligned(q_out, 16) || !aligned(k_out, 16) ||
+      !aligned(v_out, 16) || !aligned(slots, 8) || strides[0] * bytes % 16 != 0 || strides[1] * bytes % 16 != 0 || strides[2] * bytes % 16 != 0)
+    return FMHA_I8_ERR_MISALIGNED;
+  rope::Params p{};
+  if (slots) {
+    if (cache[0] < 1 || !power_of_two(cache[1]) || cache[1] < 16 || cache[1] > 4096 || cache[2] < Hkv * cache[1] * D) return FMHA_I8_ERR_BAD_SHAPE;
+    if (cache[0] > 0x7FFFFFFELL) return FMHA_I8_ERR_TOO_LARGE;
+    if (cache[2] % 16 != 0) return FMHA_I8_ERR_MISALIGNED;
+    p.page_shift = log2_of(cache[1]);
+    p.page_stride = cache[2];
+    p.num_slots = cache[0] * cache[1];
+  }
+  p.q = q; p.k = k; p.v = v;
+  p.q_out = q_out; p.k_out = k_out; p.v_out = v_out;
+  p.positions = positions;
+  p.table = table;
+  p.slots = slots;
+  p.in_table = in_table;
+  p.q_stride = strides[0]; p.k_stride = strides[1]; p.v_stride = strides[2];
+  p.tokens = static_cast<int>(tokens);
+  p.H = static_cast<int>(H);
+  p.Hkv = static_cast<int>(Hkv);
+  p.rot = static_cast<int>(rot);
+  p.interleaved = interleaved != 0;
+  for (int i = 0; i < 3; ++i) { p.amax[i] = amax[i]; p.scale[i] = 127.f / amax[i]; }
+  Device dev;
+  int st = fmha_host::device_for_call(&dev);
+  if (st != FMHA_I8_OK || tokens == 0) return st;
+  p.status = dev.status;
+  p.host_word = dev.host_word;
+  // Warps that take one round of heads each, as long as that does not make more than the chip holds at once.
+  const int at_once = static_cast<int>(512 / D), all = static_cast<int>((H + 2 * Hkv + at_once - 1) / at_once);
+  const long long most_warps = 48LL * dev.sm_count;
+  p.rounds = static_cast<int>(std::min<long long>(all, std::max<long long>(1, (tokens * all + most_warps - 1) / most_warps)));
+  p.parts = (all + p.rounds - 1) / p.rounds;
+  const long long blocks = (tokens * p.parts + rope::kThreads / 32 - 1) / (rope::kThreads / 32);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const unsigned grid = static_cast<unsigned>(blocks);
+  if (in_type == FMHA_I8_TYPE_BF16) return launch_append<__nv_bfloat16>(s, p, static_cast<int>(D), grid);
+  if (in_type == FMHA_I8_TYPE_FP16) return launch_append<__half>(s, p, static_cast<int>(D), grid);
+  return launch_append<float>(s, p, static_cast<int>(D), grid);
+}
+
+}  // namespace
+
+extern "C" {
+
+int fmha_i8_sm100_infer_packed(void* stream, const float amax[5], const int desc6[6], const void* q, const void* k, const void* v,
+                               const int* cu_seqlens_q, const int* cu_seqlens_k, void* o, int o_type, const long long tokens[2],
+                               const long long strides[4], unsigned flags) {
+  return finish(infer_packed_impl(stream, amax, desc6, q, k, v, cu_seqlens_q, cu_seqlens_k, o, o_type, tokens, strides, flags));
+}
+
+int fmha_i8_sm100_infer_paged(void* stream, const float amax[5], const int desc6[6], const void* q, const void* k_cache, const void* v_cache,
+                              const int* page_table, const int* seqlens_k, const int* cu_seqlens_q, void* o, int o_type, long long tokens,
+                              const long long strides[2], const long long cache[5], unsigned flags) {
+  return finish(infer_paged_impl(stream, amax, desc6, q, k_cache, v_cache, page_table, seqlens_k, cu_seqlens_q, o, o_type, tokens, strides, cache, flags));
+}
+
+int fmha_i8_sm100_rope_table(void* stream, const double* inv_freq, int pairs, long long positions, double magnitude, float* table) {
+  return finish(rope_table_impl(stream, inv_freq, pairs, positions, magnitude, table));
+}
+
+int fmha_i8_sm100_rope_quantize_append(void* stream, const float amax[5], const long long dims[5], const void* q, const void* k, const void* v, int in_type,
+                                       const long long strides[3], const int* positions, const float* table, long long positions_in_table,
+                                       int interleaved, int8_t* q_out, int8_t* k_out, int8_t* v_out, const long long* slots, const long long cache[3]) {
+  return finish(append_impl(stream, amax, dims, q, k, v, in_type, strides, positions, table, positions_in_table, interleaved, q_out, k_out, v_out, slots, cache));
+}
+
+}  // extern "C"

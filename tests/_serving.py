@@ -1,0 +1,95 @@
+"""64-bit references of the serving calls and the tolerances that follow from their roundings (numpy, or torch on any device)."""
+import math
+
+import torch
+
+TYPES = {"int8": torch.int8, "bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+AMAX = (4.5, 4.75, 4.25)
+
+
+def codes(shape, seed, device="cuda"):
+    """Every int8 code that the quantiser gives, evenly."""
+    g = torch.Generator(device=device)
+    g.manual_seed(seed)
+    return torch.randint(-127, 128, shape, dtype=torch.int8, device=device, generator=g)
+
+
+def starts(lengths, device="cuda"):
+    at = [0]
+    for n in lengths:
+        at.append(at[-1] + n)
+    return torch.tensor(at, dtype=torch.int32, device=device)
+
+
+def attention64(q, k, v, amax, causal):
+    """One sequence: q [n, H, D], k, v [m, Hkv, D] int8 -> (o, spread) float64 [n, H, D]: the output in real units and the tolerance's
+    scale, sum_j p_j |v_j| (see tolerance())."""
+    n, H, D = q.shape
+    m, Hkv = k.shape[0], k.shape[1]
+    if n == 0 or m == 0:
+        return (torch.zeros((n, H, D), dtype=torch.float64, device=q.device),) * 2
+    scale = float(torch.tensor(amax[0])) * float(torch.tensor(amax[1])) / 127.0 ** 2 / math.sqrt(D)
+    kk, vv = (x.double().repeat_interleave(H // Hkv, 1).transpose(0, 1) for x in (k, v))
+    s = q.double().transpose(0, 1) @ kk.transpose(1, 2) * scale
+    seen = torch.ones((n, m), dtype=torch.bool, device=q.device)
+    if causal:
+        seen = seen.tril(m - n)
+    s = s.masked_fill(~seen, -math.inf)
+    top = s.amax(-1, keepdim=True)
+    p = torch.exp(s - torch.where(top == -math.inf, 0.0, top))
+    l = p.sum(-1, keepdim=True)
+    p = torch.where(l > 0, p / torch.where(l > 0, l, 1.0), 0.0)
+    real = float(torch.tensor(amax[2])) / 127.0
+    return (p @ vv).transpose(0, 1) * real, (p @ vv.abs()).transpose(0, 1) * real
+
+
+def tolerance(o, spread, keys, o_type, amax, o_amax):
+    """Elementwise bound of |result - o|, o in real units.
+      P        fp16: half a step, 2^-11 relative, of every p: 2^-11 sum p |v|; below 2^-14 half a step is 2^-25 of the largest p (which is 2^-8 at the least
+               where the exponent's reference is kept while a row's maximum grows by less than 2^8, or is rounded): 2^-17 |v| per key, of sum p >= 1
+               times that, i.e. at most keys * 2^-25 / 2^-8 * v_amax where rows are that uneven; rows here are not: the sum of p is at
+               least the largest p, and 2^-25 * keys * v_amax is what is allowed.
+      exp2     2^-22, its argument (|a| <= 24 where p matters to fp16) rounded to 2^-24 relative: 24 * 2^-24 < 2^-19 together.
+      sums     keys additions in fp32, half a step (2^-24) each, of sums at most sum p |v|.
+      output   half a step of its type relative to the result (int8: half a code)."""
+    out = torch.full_like(o, 0.5 * o_amax / 127.0) if o_type == "int8" else o.abs() * (torch.finfo(TYPES[o_type]).eps / 2)
+    tiny = 0.0 if o_type != "fp16" else 2.0 ** -25            # half a step below fp16's smallest normal number
+    return out * 1.001 + spread * (2.0 ** -11 + 2.0 ** -18 + keys * 2.0 ** -24) + keys * 2.0 ** -25 * amax[2] + tiny
+
+
+def real_units(o, o_type, o_amax):
+    return o.double() * (o_amax / 127.0) if o_type == "int8" else o.double()
+
+
+def check(got, want, spread, keys, o_type, amax, o_amax, what=""):
+    want_c = want.clamp(-o_amax, o_amax) if o_type == "int8" else want
+    err = (real_units(got, o_type, o_amax) - want_c).abs()
+    tol = tolerance(want_c, spread, keys, o_type, amax, o_amax)
+    over = err > tol
+    assert not bool(over.any()), f"{what}: {int(over.sum())} of {over.numel()} off, worst {float((err / tol).max()):.3g} times the tolerance"
+
+
+def rotate64(x, positions, inv_freq, magnitude, interleaved):
+    """x float64 [T, heads, D]."""
+    half = inv_freq.numel()
+    if half == 0:
+        return x
+    angle = positions.double()[:, None] * inv_freq.double()
+    c, s = (torch.cos(angle) * magnitude)[:, None], (torch.sin(angle) * magnitude)[:, None]
+    y = x.clone()
+    a, b = (slice(0, 2 * half, 2), slice(1, 2 * half, 2)) if interleaved else (slice(0, half), slice(half, 2 * half))
+    y[..., a] = x[..., a] * c - x[..., b] * s
+    y[..., b] = x[..., b] * c + x[..., a] * s
+    return y
+
+
+def quantise64(y, amax):
+    """clamp(floor(y * (127 / amax) + 1/2), -127, 127); not a number gives 0."""
+    z = torch.floor(y * (127.0 / float(torch.tensor(amax, dtype=torch.float32))) + 0.5).clamp(-127, 127)
+    return torch.nan_to_num(z, nan=0.0).to(torch.int8)
+
+
+def assert_same(got, want):
+    assert got.shape == want.shape
+    off = int((got != want).sum())
+    assert off == 0, f"{off} of {want.numel()} codes differ"
