@@ -38,6 +38,7 @@ struct Params {
   int total_q, total_k, max_q;
   int o_type, causal;
   int row_groups;                      // rows kernel: groups of 16 rows per sequence and key head
+  int tq;                              // chunk kernel: tokens per tile of 128 rows
   float c2;                            // from a difference of scores to an exponent of 2
   float out_scale;                     // from sum p v / sum p, v in codes, to the output's unit
   unsigned* status;                    // eight device status words

@@ -5,10 +5,12 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <cstdio>
 #include <mutex>
 #include <utility>
 
 #include "../../include/fmha_i8_c.h"
+#include "fmha_chunk_sm100.cuh"
 #include "fmha_grouped_sm100.cuh"
 #include "fmha_internal.h"
 #include "fmha_rope_sm100.cuh"
@@ -87,6 +89,20 @@ template <int D> int set_up_rows(int* clusters16) {
   return FMHA_I8_OK;
 }
 
+template <int D> int set_up_chunk() {
+  const void* fn = reinterpret_cast<const void*>(&chunk::chunk_kernel<D>);
+  cudaFuncAttributes fa{};
+  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(chunk::smem_bytes<D>())) != cudaSuccess ||
+      cudaFuncGetAttributes(&fa, fn) != cudaSuccess) {
+    cudaGetLastError();
+    return FMHA_I8_ERR_LAUNCH;
+  }
+  // the kernel moves registers between its warps with setmaxnreg, which only terminates if the launch allocation is what the targets were sized for
+  if (fa.numRegs == chunk::kLaunchRegs) return FMHA_I8_OK;
+  std::fprintf(stderr, "fmha_i8_sm100: chunk kernel built with %d registers per thread, expected %d; refusing to launch\n", fa.numRegs, chunk::kLaunchRegs);
+  return FMHA_I8_ERR_LAUNCH;
+}
+
 int set_up(const Device& dev) {
   Once& once = g_once[dev.index];
   if (once.done.load(std::memory_order_acquire)) return FMHA_I8_OK;
@@ -95,6 +111,7 @@ int set_up(const Device& dev) {
   int st;
   if ((st = set_up_rows<64>(&once.clusters16_d64)) != FMHA_I8_OK) return st;
   if ((st = set_up_rows<128>(&once.clusters16_d128)) != FMHA_I8_OK) return st;
+  if ((st = set_up_chunk<64>()) != FMHA_I8_OK || (st = set_up_chunk<128>()) != FMHA_I8_OK) return st;
   once.done.store(true, std::memory_order_release);
   return FMHA_I8_OK;
 }
@@ -177,6 +194,28 @@ template <int D> int launch_rows(cudaStream_t stream, const Device& dev, Call& c
   return launch(rows::rows_kernel<D, W>, static_cast<unsigned>(units * ctas), W * 32, sizeof(rows::Smem<D, W>), stream, static_cast<unsigned>(ctas), mk, mv, p);
 }
 
+// Up to 128 heads share a key head, and a tile of the chunk kernel holds at least one token.
+constexpr int kMostGroup = 128;
+bool few_rows(const grouped::Params& p) { return p.G > kMostGroup || static_cast<long long>(p.max_q) * p.G <= rows::kRows; }
+
+template <int D> int launch_chunk(cudaStream_t stream, const Device& dev, Call& c, const CUtensorMap& mk, const CUtensorMap& mv) {
+  grouped::Params& p = c.p;
+  p.tq = grouped::kTile / p.G;
+  auto fn = fmha_host::encode_tiled();
+  CUtensorMap mq;
+  const cuuint64_t dims[3] = {D, static_cast<cuuint64_t>(p.H), static_cast<cuuint64_t>(p.total_q)};
+  const cuuint64_t strides[2] = {D, static_cast<cuuint64_t>(p.q_stride)};
+  const cuuint32_t box[3] = {D, static_cast<cuuint32_t>(p.G), static_cast<cuuint32_t>(p.tq)}, ones[3] = {1u, 1u, 1u};
+  if (!fn || fn(&mq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<int8_t*>(p.q), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return FMHA_I8_ERR_DRIVER;
+  // pairs of tiles: no more than the tokens make, and one more for every sequence
+  const long long units = std::min<long long>(p.total_q, p.total_q / (2LL * p.tq) + p.B) * p.Hkv;
+  if (units > kMostRows) return FMHA_I8_ERR_TOO_LARGE;
+  const unsigned grid = static_cast<unsigned>(std::min<long long>(units, dev.sm_count));
+  return launch(chunk::chunk_kernel<D>, grid, chunk::kThreads, chunk::smem_bytes<D>(), stream, 0u, mq, mk, mv, p);
+}
+
 int run_attention(void* stream, Call& c) {
   Device dev;
   int st;
@@ -189,7 +228,8 @@ int run_attention(void* stream, Call& c) {
   if ((st = key_map(&mk, c.k, c.lk, c.D)) != FMHA_I8_OK) return st;
   if ((st = key_map(&mv, c.v, c.lv, c.D)) != FMHA_I8_OK) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return c.D == 128 ? launch_rows<128>(s, dev, c, mk, mv) : launch_rows<64>(s, dev, c, mk, mv);
+  if (few_rows(c.p)) return c.D == 128 ? launch_rows<128>(s, dev, c, mk, mv) : launch_rows<64>(s, dev, c, mk, mv);
+  return c.D == 128 ? launch_chunk<128>(s, dev, c, mk, mv) : launch_chunk<64>(s, dev, c, mk, mv);
 }
 
 int infer_packed_impl(void* stream, const float amax[5], const int desc6[6], const void* q, const void* k, const void* v, const int* cu_q, const int* cu_k, void* o,
