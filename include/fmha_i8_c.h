@@ -62,6 +62,7 @@ enum {
   FMHA_I8_DEV_WAIT_DEBUG = 10,     /* a wait inside a debug kernel */
   FMHA_I8_DEV_WAIT_INFO = 11,      /* a role waiting for (or the scanner waiting to reuse) a unit's mask information */
   FMHA_I8_DEV_WAIT_QUANT = 12,     /* quantiser: a tile of the tensor */
+  FMHA_I8_DEV_WAIT_S_FREE = 14,    /* MMA issuer waiting for the scores before to be read */
   /* No wait, but an index in device memory that points outside its tensor (nothing was accessed there): words[2] = 0: lengths or offsets of
    * sequence words[3]; 1: a page of sequence words[3]; 2: position or slot of token words[3]. */
   FMHA_I8_DEV_BAD_INDEX = 13

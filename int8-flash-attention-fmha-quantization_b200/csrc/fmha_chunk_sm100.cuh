@@ -4,17 +4,17 @@
 //   unit     = one key head and two neighbouring tiles A, B of 128 query rows of one sequence.  A row is (token, head of the group), so a tile is
 //              128 / G tokens, all G heads that share the keys; both tiles share every key tile that is brought in.
 //   persistent: one CTA per SM walks units; the longest ones come first.
-//   warps 0-3, 4-7   softmax of tile A, of tile B: one thread per row, its 128 scores in registers
+//   warps 0-3, 4-7   softmax of tile A, of tile B: one thread per row, the 128 scores of a key tile in registers
 //   warps 8-11       turn V from int8 into fp16, once for both tiles
 //   warp 12          TMA loads: Q once per unit (two buffers), rings of K and V
-//   warp 13          issues all MMAs:  S = Q K^T (kind::i8, exact),  O += P V (kind::f16, P from tensor memory)
+//   warp 13          issues S = Q K^T (kind::i8, exact)
+//   warp 15          issues O += P V (kind::f16, P from tensor memory)
 //   warp 14          turns unit numbers into sequences, tiles and key ranges, ahead of the others
 //
-// Per tile S(j+1) is issued behind P.V(j), into the columns that P(j) occupied; while one tile's softmax runs, the other's products do.
 // The output stays in tensor memory for a whole unit: a row's exponentials are taken relative to a reference that follows the running
-// maximum only when that has grown by more than 2^8, which fp16 holds easily, and then the output is rescaled in place.  That is rare
+// maximum only when that has grown by more than 2^13, which fp16 holds, and then the output is rescaled in place.  That is rare
 // behind a row's first keys.
-// Tensor memory (512 columns): S of A, S of B (128 each; P as fp16 over the first 64), O of A, O of B (128 each).
+// Tensor memory (512 columns): S of A, of B (128 columns each; P as fp16 over the first 64), O of A, of B (128 each).
 #pragma once
 #include "fmha_grouped_sm100.cuh"
 
@@ -25,14 +25,15 @@ using namespace grouped;
 
 constexpr int kThreads = 512;
 constexpr int kLaunchRegs = 128;
-constexpr int kSoftmaxRegs = 184, kConvertRegs = 80, kOtherRegs = 64;
+constexpr int kSoftmaxRegs = 200, kConvertRegs = 56, kOtherRegs = 56;
 static_assert(2 * kSoftmaxRegs + kConvertRegs + kOtherRegs <= 4 * kLaunchRegs, "setmaxnreg targets exceed the CTA's register allocation: the kernel would hang");
-constexpr int kWarpConvert = 8, kWarpLoad = 12, kWarpMma = 13, kWarpWalk = 14;
+constexpr int kWarpConvert = 8, kWarpLoad = 12, kWarpScore = 13, kWarpWalk = 14, kWarpOutput = 15;
 constexpr int kInfos = 4;
-constexpr int kInfoConsumers = 8 + 4 + 1 + 1;      // softmax warps, converters, loader, issuer
+constexpr int kInfoConsumers = 8 + 4 + 1 + 2;      // softmax warps, converters, loader, issuers
 constexpr uint32_t kTmemCols = 512;
-constexpr int kMasked = static_cast<int>(0xFF800000u - kMagicBits);      // a score that reads as minus infinity once kMagicBits are added
-constexpr int kLowest = -(1 << 22);                                      // below every score
+constexpr int kLowest = -(1 << 22);                                      // below every score (127 * 127 * 128 < 2^21)
+// A score that, with kMagicBits and less any other score, is the bits of a float of about -2^127, whose exponential is zero.
+constexpr int kMasked = static_cast<int>(0xFF000000u - kMagicBits);
 
 template <int D> struct Cfg {
   static constexpr int kTileBytes = kTile * D;
@@ -45,6 +46,7 @@ template <int D> struct Cfg {
 struct Steps {
   int valid;
   int n[2];             // key tiles of A, of B
+  __device__ __forceinline__ int all() const { return max(n[0], n[1]); }
 };
 struct Unit : Steps {
   Seq seq;
@@ -56,7 +58,9 @@ template <int D> struct Ctl {
   using C = Cfg<D>;
   uint64_t info_full[kInfos], info_empty[kInfos];
   uint64_t q_full[2], q_empty[2], k_full[C::kStagesK], k_empty[C::kStagesK], v_full[C::kStagesV], v_empty[C::kStagesV], h_full[C::kStagesH], h_empty[C::kStagesH];
-  uint64_t s_full[2], p_ready[2], o_full[2], o_free[2];      // per tile
+  uint64_t s_full[2], s_read[2];                     // per tile: the scores of a step are there, and in registers
+  uint64_t p_ready[2][2];                            // per tile: either half of P
+  uint64_t o_full[2], o_free[2];                     // per tile: the unit's output is complete, and has been read
   uint32_t tmem_base;
   int abort;
   Unit unit[kInfos];
@@ -67,14 +71,29 @@ template <int D> constexpr size_t smem_bytes() { return 1024 + Cfg<D>::kBytes + 
 template <int D> struct UnitReader {
   Ctl<D>* ctl;
   uint32_t n = 0;
-  template <typename T> __device__ __forceinline__ bool next(T& u) {       // a Unit or its Steps
-    const uint32_t slot = n % kInfos;
-    if (!warp_wait(smem_u32(&ctl->info_full[slot]), (n / kInfos) & 1u, &ctl->abort)) return false;
-    u = static_cast<const T&>(ctl->unit[slot]);
-    __syncwarp();
-    if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(&ctl->info_empty[slot]));
-    ++n;
+  __device__ __forceinline__ bool next(Unit& u) {
+    if (!wait()) return false;
+    u = here();
+    release();
     return true;
+  }
+  // For those who need no more.  They see the numbers as uniform values (see uniform()).
+  __device__ __forceinline__ bool next(Steps& u) {
+    if (!wait()) return false;
+    const Unit& x = here();
+    u.valid = uniform(x.valid);
+    u.n[0] = uniform(x.n[0]);
+    u.n[1] = uniform(x.n[1]);
+    release();
+    return true;
+  }
+  // The same in two steps, for those who leave it where it is: here() until release().
+  __device__ __forceinline__ bool wait() { return warp_wait(smem_u32(&ctl->info_full[n % kInfos]), (n / kInfos) & 1u, &ctl->abort); }
+  __device__ __forceinline__ const Unit& here() const { return ctl->unit[n % kInfos]; }
+  __device__ __forceinline__ void release() {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(&ctl->info_empty[n % kInfos]));
+    ++n;
   }
 };
 
@@ -170,7 +189,7 @@ template <int D> __device__ __forceinline__ void load_role(const Params& p, Ctl<
   while (true) {
     if (!units.next(u)) return fail(FMHA_I8_DEV_WAIT_INFO, g);
     if (!u.valid) return;
-    const int n = max(u.n[0], u.n[1]);
+    const int n = u.all();
     if (n == 0) continue;
     bool bad_page = false;
     const uint32_t buf = nq & 1u;
@@ -224,7 +243,7 @@ template <int D> __device__ __forceinline__ void convert_role(const Params& p, C
   while (true) {
     if (!units.next(u)) return fail(FMHA_I8_DEV_WAIT_INFO, g);
     if (!u.valid) return;
-    const int n = max(u.n[0], u.n[1]);
+    const int n = u.all();
     for (int j = 0; j < n; ++j, ++g) {
       const uint32_t st = g % C::kStagesV, sh = g % C::kStagesH;
       if (!warp_wait(smem_u32(&ctl->v_full[st]), (g / C::kStagesV) & 1u, abort_flag)) return fail(FMHA_I8_DEV_WAIT_V_LOAD, g);
@@ -258,75 +277,127 @@ template <int D> __device__ __forceinline__ void convert_role(const Params& p, C
 }
 
 // ------------------------------------------------------------------------------------------------ MMAs
-template <int D> __device__ __forceinline__ void mma_role(const Params& p, Ctl<D>* ctl, uint32_t smem, uint32_t tmem) {
+// Two warps issue them, each going through the steps of both tiles in turn.  Their code is kept small and is not unrolled over tiles: it runs
+// once per step between others' code, and what it took was above all the fetching of its instructions (one warp for both products, unrolled: 1425
+// cycles for a step of one tile, of which the tensor core is busy 450).
+// P of a step takes the first half of the columns of its scores.  The scores of the next step's last 64 keys therefore follow as soon as these are in
+// registers (one warp), those of the first 64 behind the P.V that reads P (the other: MMAs of one thread execute in order).
+template <int D> __device__ __forceinline__ void issue_scores(uint32_t dst, uint64_t dq, uint64_t dk) {
+  constexpr uint32_t kIdescS = make_idesc_i8(kTile / 2, false);
+#pragma unroll
+  for (int y = 0; y < D / 32; ++y) mma_i8_ss(dst, desc_advance(dq, 32 * y), desc_advance(dk, 32 * y), kIdescS, y > 0);
+}
+template <int D> __device__ __forceinline__ void score_role(const Params& p, Ctl<D>* ctl, uint32_t smem, uint32_t tmem) {
   using C = Cfg<D>;
-  constexpr uint32_t kIdescS = make_idesc_i8(kTile, false), kIdescO = make_idesc_f16_b_mn(D);
   const Failure fail{p, &ctl->abort};
   volatile int* abort_flag = &ctl->abort;
   UnitReader<D> units{ctl};
-  Steps cur, next;
-  uint32_t g = 0, nq = 0;                            // key tiles and units with keys before the present unit
-  uint32_t steps[2] = {0, 0}, outs[2] = {0, 0};      // P.V issued, units begun, per tile
-  // S of tile t, step j of a unit whose first key tile is g0 and which is the n-th with keys
-  auto issue_s = [&](const Steps& u, int t, int j, uint32_t g0, uint32_t n) -> bool {
-    const uint32_t gj = g0 + static_cast<uint32_t>(j), st = gj % C::kStagesK, buf = n & 1u;
-    if (j == 0 && !warp_wait(smem_u32(&ctl->q_full[buf]), (n >> 1) & 1u, abort_flag)) { fail(FMHA_I8_DEV_WAIT_Q_LOAD, n); return false; }
-    if (!warp_wait(smem_u32(&ctl->k_full[st]), (gj / C::kStagesK) & 1u, abort_flag)) { fail(FMHA_I8_DEV_WAIT_K_LOAD, gj); return false; }
-    tc_fence_after();
-    const uint64_t dq = make_smem_desc(smem + C::kQ + (2 * buf + t) * C::kTileBytes, D), dk = make_smem_desc(smem + C::kK + st * C::kTileBytes, D);
-    const int all = max(u.n[0], u.n[1]);
-    if (elect_one()) {
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) mma_i8_ss(tmem + t * kTile, desc_advance(dq, 32 * i), desc_advance(dk, 32 * i), kIdescS, i > 0);
-      mma_commit(smem_u32(&ctl->s_full[t]));
-      if (t == (j < u.n[1] ? 1 : 0)) {               // the last one to read this K tile
-        mma_commit(smem_u32(&ctl->k_empty[st]));
-        if (j == all - 1) mma_commit(smem_u32(&ctl->q_empty[buf]));
-      }
-    }
-    __syncwarp();
-    return true;
-  };
-  if (!units.next(cur)) return fail(FMHA_I8_DEV_WAIT_INFO, 0);
-  if (!cur.valid) return;
-  bool ok = true;
-#pragma unroll
-  for (int t = 0; t < 2; ++t)
-    if (ok && cur.n[t] > 0) ok = issue_s(cur, t, 0, g, nq);
-  while (ok) {
-    if (!units.next(next)) return fail(FMHA_I8_DEV_WAIT_INFO, g);
-    const int all = max(cur.n[0], cur.n[1]);
-    const uint32_t g_next = g + static_cast<uint32_t>(all), nq_next = nq + (all > 0);
-    for (int j = 0; j < max(all, 1) && ok; ++j) {
-#pragma unroll
+  Steps u;
+  uint32_t st = 0, k_phase = 0, nq = 0;              // K stage and its phase, units with keys
+  uint32_t count_a = 0, count_b = 0;                 // steps issued for A, for B
+  while (true) {
+    if (!units.next(u)) return fail(FMHA_I8_DEV_WAIT_INFO, count_a);
+    if (!u.valid) return;
+    const int all = u.all();
+    if (all == 0) continue;
+    const uint32_t q = nq & 1u;
+    if (!warp_wait(smem_u32(&ctl->q_full[q]), (nq >> 1) & 1u, abort_flag)) return fail(FMHA_I8_DEV_WAIT_Q_LOAD, nq);
+    ++nq;
+#pragma unroll 1
+    for (int i = 0; i < all; ++i) {
+      if (!warp_wait(smem_u32(&ctl->k_full[st]), k_phase, abort_flag)) return fail(FMHA_I8_DEV_WAIT_K_LOAD, i);
+      const uint64_t dk = make_smem_desc(smem + C::kK + st * C::kTileBytes + C::kTileBytes / 2, D);
+#pragma unroll 1
       for (int t = 0; t < 2; ++t) {
-        if (!ok) break;
-        if (j < cur.n[t]) {
-          const uint32_t gj = g + static_cast<uint32_t>(j), sh = gj % C::kStagesH;
-          if (j == 0 && outs[t] > 0 && !warp_wait(smem_u32(&ctl->o_free[t]), (outs[t] - 1) & 1u, abort_flag)) { fail(FMHA_I8_DEV_WAIT_O_FREE, gj); return; }
-          if (!warp_wait(smem_u32(&ctl->h_full[sh]), (gj / C::kStagesH) & 1u, abort_flag)) { fail(FMHA_I8_DEV_WAIT_V_LOAD, gj); return; }
-          if (!warp_wait(smem_u32(&ctl->p_ready[t]), steps[t] & 1u, abort_flag)) { fail(FMHA_I8_DEV_WAIT_P_READY, gj); return; }
-          tc_fence_after();
-          const uint64_t dv = make_smem_desc_slabs(smem + C::kH + sh * C::kHalfBytes, C::kHalfBytes / 2);
-          if (elect_one()) {
+        if (i >= (t ? u.n[1] : u.n[0])) continue;
+        const uint32_t c = t ? count_b++ : count_a++;
+        if (c > 0 && !warp_wait(smem_u32(&ctl->s_read[t]), (c - 1) & 1u, abort_flag)) return fail(FMHA_I8_DEV_WAIT_S_FREE, c);
+        tc_fence_after();
+        if (elect_one()) {
+          issue_scores<D>(tmem + t * kTile + kTile / 2, make_smem_desc(smem + C::kQ + (2 * q + t) * C::kTileBytes, D), dk);
+          mma_commit(smem_u32(&ctl->s_full[t]));
+        }
+        __syncwarp();
+      }
+      if (elect_one()) mma_commit(smem_u32(&ctl->k_empty[st]));
+      __syncwarp();
+      if (++st == C::kStagesK) { st = 0; k_phase ^= 1u; }
+    }
+    if (elect_one()) mma_commit(smem_u32(&ctl->q_empty[q]));
+    __syncwarp();
+  }
+}
+
+template <int D> __device__ __forceinline__ void output_role(const Params& p, Ctl<D>* ctl, uint32_t smem, uint32_t tmem) {
+  using C = Cfg<D>;
+  constexpr uint32_t kIdescO = make_idesc_f16_b_mn(D);
+  const Failure fail{p, &ctl->abort};
+  volatile int* abort_flag = &ctl->abort;
+  UnitReader<D> units{ctl};
+  Steps u;
+  uint32_t st = 0, k_phase = 0, sh = 0, h_phase = 0, nq = 0;
+  uint32_t count_a = 0, count_b = 0, outs_a = 0, outs_b = 0;      // steps issued and units begun for A, for B
+  while (true) {
+    if (!units.next(u)) return fail(FMHA_I8_DEV_WAIT_INFO, count_a);
+    if (!u.valid) return;
+    const int all = u.all();
+    if (all == 0) continue;
+    const uint32_t q = nq & 1u;
+    if (!warp_wait(smem_u32(&ctl->q_full[q]), (nq >> 1) & 1u, abort_flag)) return fail(FMHA_I8_DEV_WAIT_Q_LOAD, nq);
+    ++nq;
+    // Step i: P.V of key tile i (none for i = -1), then the scores of the first 64 keys of tile i + 1.
+#pragma unroll 1
+    for (int i = -1; i < all; ++i) {
+      if (i >= 0 && !warp_wait(smem_u32(&ctl->h_full[sh]), h_phase, abort_flag)) return fail(FMHA_I8_DEV_WAIT_V_LOAD, i);
+      if (i + 1 < all && !warp_wait(smem_u32(&ctl->k_full[st]), k_phase, abort_flag)) return fail(FMHA_I8_DEV_WAIT_K_LOAD, i);
+      const uint64_t dv0 = make_smem_desc_slabs(smem + C::kH + sh * C::kHalfBytes, C::kHalfBytes / 2);
+      const uint64_t dk = make_smem_desc(smem + C::kK + st * C::kTileBytes, D);
+#pragma unroll 1
+      for (int t = 0; t < 2; ++t) {
+        const int n = t ? u.n[1] : u.n[0];
+        if (i >= n) continue;
+        if (i >= 0) {
+          const uint32_t c = t ? count_b++ : count_a++;
+          if (i == 0) {
+            const uint32_t outs = t ? outs_b++ : outs_a++;
+            if (outs > 0 && !warp_wait(smem_u32(&ctl->o_free[t]), (outs - 1) & 1u, abort_flag)) return fail(FMHA_I8_DEV_WAIT_O_FREE, outs);
+          }
+#pragma unroll 1
+          for (int upper = 0; upper < 2; ++upper) {
+            if (!warp_wait(smem_u32(&ctl->p_ready[t][upper]), c & 1u, abort_flag)) return fail(FMHA_I8_DEV_WAIT_P_READY, c);
+            tc_fence_after();
+            if (elect_one()) {
 #pragma unroll
-            for (int i = 0; i < kTile / 16; ++i)
-              mma_f16_ts(tmem + 2 * kTile + t * kTile, tmem + t * kTile + 8 * i, desc_advance(dv, 16 * 128 * i), kIdescO, j > 0 || i > 0);
-            if (t == (j < cur.n[1] ? 1 : 0)) mma_commit(smem_u32(&ctl->h_empty[sh]));
-            if (j == cur.n[t] - 1) mma_commit(smem_u32(&ctl->o_full[t]));
+              for (int y = 0; y < kTile / 32; ++y)
+                mma_f16_ts(tmem + 2 * kTile + t * kTile, tmem + t * kTile + upper * (kTile / 4) + 8 * y, desc_advance(dv0, upper * (kTile / 2 * 128) + 16 * 128 * y), kIdescO,
+                           i > 0 || upper > 0 || y > 0);
+              if (upper && i == n - 1) mma_commit(smem_u32(&ctl->o_full[t]));
+            }
+            __syncwarp();
+          }
+        }
+        if (i + 1 < n) {
+          tc_fence_after();
+          if (elect_one()) {
+            issue_scores<D>(tmem + t * kTile, make_smem_desc(smem + C::kQ + (2 * q + t) * C::kTileBytes, D), dk);
+            mma_commit(smem_u32(&ctl->s_full[t]));
           }
           __syncwarp();
-          ++steps[t];
-          if (j == 0) ++outs[t];
         }
-        if (j + 1 < cur.n[t]) ok = issue_s(cur, t, j + 1, g, nq);
-        else if (j == max(all, 1) - 1 && next.valid && next.n[t] > 0) ok = issue_s(next, t, 0, g_next, nq_next);
+      }
+      if (i >= 0) {
+        if (elect_one()) mma_commit(smem_u32(&ctl->h_empty[sh]));    // both tiles have read this V tile
+        __syncwarp();
+        if (++sh == C::kStagesH) { sh = 0; h_phase ^= 1u; }
+      }
+      if (i + 1 < all) {
+        if (elect_one()) mma_commit(smem_u32(&ctl->k_empty[st]));
+        __syncwarp();
+        if (++st == C::kStagesK) { st = 0; k_phase ^= 1u; }
       }
     }
-    if (!next.valid) return;
-    cur = next;
-    g = g_next;
-    nq = nq_next;
+    if (elect_one()) mma_commit(smem_u32(&ctl->q_empty[q]));
+    __syncwarp();
   }
 }
 
@@ -334,98 +405,116 @@ template <int D> __device__ __forceinline__ void mma_role(const Params& p, Ctl<D
 __device__ __forceinline__ int max3(int a, int b, int c) { return __vimax3_s32(a, b, c); }
 
 template <int D> __device__ __forceinline__ void softmax_role(const Params& p, Ctl<D>* ctl, uint32_t tmem) {
-  const int warp = warp_index(), t = warp >> 2, lane = threadIdx.x & 31;
-  const int row = (warp & 3) * 32 + lane;
+  const int warp = warp_index(), t = warp >> 2, quad = warp & 3, lane = threadIdx.x & 31;
+  const int row = quad * 32 + lane;
   const Failure fail{p, &ctl->abort};
   volatile int* abort_flag = &ctl->abort;
-  const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+  const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
   const uint32_t tS = tmem + lanes + t * kTile, tO = tmem + lanes + 2 * kTile + t * kTile;
-  const int my_token = row / p.G, my_head = row - my_token * p.G;
-  const float2 c2 = make_float2(p.c2, p.c2);
+  const int my_token = row / p.G;
+  const float2 c2 = make_float2(p.c2, p.c2), less = make_float2(-kMagic * p.c2, -kMagic * p.c2);
   UnitReader<D> units{ctl};
-  Unit u;
   uint32_t steps = 0, outs = 0;
   while (true) {
-    if (!units.next(u)) return fail(FMHA_I8_DEV_WAIT_INFO, steps);
+    if (!units.wait()) return fail(FMHA_I8_DEV_WAIT_INFO, steps);
+    const Unit& u = units.here();
     if (!u.valid) return;
-    const int token = u.token0 + t * p.tq + my_token;
-    const bool real = my_token < p.tq && token < u.seq.nq;
-    const int n = u.n[t];
-    const int limit = real ? visible(p, u.seq, token) : 0;
+    const int n = uniform(u.n[t]);
+    bool real;
+    int limit;
+    {
+      const int token = u.token0 + t * p.tq + my_token;
+      real = my_token < p.tq && token < u.seq.nq;
+      limit = real ? visible(p, u.seq, token) : 0;
+    }
     const bool any = __any_sync(0xFFFFFFFFu, limit > 0);            // a warp without a row that sees a key leaves its part of P as it is
     const int least = __reduce_min_sync(0xFFFFFFFFu, real ? limit : 0x7FFFFFFF);
-    float ref = kMagic, hi = 0.f;                                  // a reference score, as the float kMagic + score, and its exponent
+    // p = 2^((s - ref) c2), with an integer ref.  kMagicBits + (s - ref) are the bits of the float kMagic + (s - ref), exactly, and c2 has so few of them that
+    // kMagic * c2 is a float too: one multiply-add gives the exponent, rounded once.
+    int ref = 0;
     float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll 1
-    for (int j = 0; j < n; ++j, ++steps) {
+    for (int i = 0; i < n; ++i, ++steps) {
       if (!warp_wait(smem_u32(&ctl->s_full[t]), steps & 1u, abort_flag)) return fail(FMHA_I8_DEV_WAIT_S_READY, steps);
-      tc_fence_after();
+      uint32_t r[8][16];
       if (any) {
-        uint32_t r[4][32];
+        tc_fence_after();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) tmem_ld32_issue(tS + 32 * i, r[i]);
+        for (int x = 0; x < 8; ++x) tmem_ld16_issue(tS + 16 * x, r[x]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) tmem_ld_fence(r[i]);
-        if (j * kTile + kTile > least) {
-          const int open = limit - j * kTile;
+        for (int x = 0; x < 8; ++x) tmem_ld_fence(r[x]);
+        tc_fence_before();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&ctl->s_read[t]));
+      if (any) {
+        if (i * kTile + kTile > least) {
+          const int open = limit - i * kTile;
 #pragma unroll
-          for (int i = 0; i < 128; ++i)
-            if (i >= open) r[i >> 5][i & 31] = static_cast<uint32_t>(kMasked);
+          for (int x = 0; x < kTile; ++x)
+            if (x >= open) r[x >> 4][x & 15] = static_cast<uint32_t>(kMasked);
         }
         int m0 = kLowest, m1 = kLowest;
 #pragma unroll
-        for (int i = 0; i < 128; i += 4) {
-          m0 = max3(m0, static_cast<int>(r[i >> 5][i & 31]), static_cast<int>(r[i >> 5][(i & 31) + 1]));
-          m1 = max3(m1, static_cast<int>(r[i >> 5][(i & 31) + 2]), static_cast<int>(r[i >> 5][(i & 31) + 3]));
+        for (int x = 0; x < kTile; x += 4) {
+          m0 = max3(m0, static_cast<int>(r[x >> 4][x & 15]), static_cast<int>(r[x >> 4][(x & 15) + 1]));
+          m1 = max3(m1, static_cast<int>(r[x >> 4][(x & 15) + 2]), static_cast<int>(r[x >> 4][(x & 15) + 3]));
         }
-        const float m = __int_as_float(max(m0, m1) + static_cast<int>(kMagicBits));
-        if (j == 0) {
+        const int m = max(m0, m1);
+        if (i == 0) {
           ref = m;
-          hi = m * p.c2;
         } else {
-          const bool grown = (m - ref) * p.c2 > 8.f;
+          const bool grown = m - ref > p.growth;
           if (__any_sync(0xFFFFFFFFu, grown)) {
-            const float next = grown ? m * p.c2 : hi, factor = grown ? ex2(hi - next) : 1.f;
+            const float factor = grown ? ex2(static_cast<float>(ref - m) * p.c2) : 1.f;
             if (grown) ref = m;
-            hi = next;
             sum[0].x *= factor; sum[0].y *= factor; sum[1].x *= factor; sum[1].y *= factor;
-            // (the last P.V of this tile was issued before the S that has just been waited for, and is complete with it)
+            // (the scores that have just been read were formed behind P.V of the step before)
 #pragma unroll 1
-            for (int i = 0; i < D; i += 16) {
+            for (int x = 0; x < D; x += 16) {
               uint32_t o[16];
-              tmem_ld16_issue(tO + i, o);
+              tmem_ld16_issue(tO + x, o);
               tmem_ld_fence(o);
 #pragma unroll
-              for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * factor);
-              tmem_st8(tO + i, reinterpret_cast<uint32_t(&)[8]>(o[0]));
-              tmem_st8(tO + i + 8, reinterpret_cast<uint32_t(&)[8]>(o[8]));
+              for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * factor);
+              tmem_st16(tO + x, o);
             }
           }
         }
-        const float2 neg = make_float2(-hi, -hi);
+      }
+      if (any) {
+        const uint32_t bits = kMagicBits - static_cast<uint32_t>(ref);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          uint32_t packed[32];
+        for (int h = 0; h < 8; ++h) {
+          uint32_t packed[8];
 #pragma unroll
-          for (int x = 0; x < 32; ++x) {
-            const int at = 64 * i + 2 * x;
-            const float2 s = make_float2(__uint_as_float(r[at >> 5][at & 31] + kMagicBits), __uint_as_float(r[at >> 5][(at & 31) + 1] + kMagicBits));
-            const float2 a = __ffma2_rn(s, c2, neg);
+          for (int x = 0; x < 8; ++x) {
+            const float2 v = make_float2(__uint_as_float(r[h][2 * x] + bits), __uint_as_float(r[h][2 * x + 1] + bits));
+            const float2 a = __ffma2_rn(v, c2, less);
             const float2 e = make_float2(ex2(a.x), ex2(a.y));
             sum[x & 1] = __fadd2_rn(sum[x & 1], e);
-            const __half2 h = __floats2half2_rn(e.x, e.y);
-            packed[x] = *reinterpret_cast<const uint32_t*>(&h);
+            const __half2 q = __floats2half2_rn(e.x, e.y);
+            packed[x] = *reinterpret_cast<const uint32_t*>(&q);
           }
-          tmem_st32(tS + 32 * i, packed);
+          if (h == 4) {                              // the first half of P; the latency of its stores lies behind the powers of this lot
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&ctl->p_ready[t][0]));
+          }
+          tmem_st8(tS + 8 * h, packed);
         }
         tmem_wait_st();
+      } else if (lane == 0) {
+        mbar_arrive(smem_u32(&ctl->p_ready[t][0]));
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&ctl->p_ready[t]));
+      if (lane == 0) mbar_arrive(smem_u32(&ctl->p_ready[t][1]));
     }
     // ---- the row's output
-    const long long at = (u.seq.q0 + token) * p.o_stride + static_cast<long long>(u.head * p.G + my_head) * D;
+    const long long at = (u.seq.q0 + u.token0 + t * p.tq + my_token) * p.o_stride + static_cast<long long>((u.head - my_token) * p.G + row) * D;
+    units.release();
     float scale = 0.f;
     if (n > 0) {
       if (!warp_wait(smem_u32(&ctl->o_full[t]), outs & 1u, abort_flag)) return fail(FMHA_I8_DEV_WAIT_O_READY, steps);
@@ -469,14 +558,16 @@ chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
   if (threadIdx.x == 0) {
     ctl->abort = 0;
     for (int i = 0; i < kInfos; ++i) { mbar_init(smem_u32(&ctl->info_full[i]), 1); mbar_init(smem_u32(&ctl->info_empty[i]), kInfoConsumers); }
-    for (int i = 0; i < C::kStagesK; ++i) { mbar_init(smem_u32(&ctl->k_full[i]), 1); mbar_init(smem_u32(&ctl->k_empty[i]), 1); }
+    for (int i = 0; i < C::kStagesK; ++i) { mbar_init(smem_u32(&ctl->k_full[i]), 1); mbar_init(smem_u32(&ctl->k_empty[i]), 2); }
     for (int i = 0; i < C::kStagesV; ++i) { mbar_init(smem_u32(&ctl->v_full[i]), 1); mbar_init(smem_u32(&ctl->v_empty[i]), 4); }
     for (int i = 0; i < C::kStagesH; ++i) { mbar_init(smem_u32(&ctl->h_full[i]), 4); mbar_init(smem_u32(&ctl->h_empty[i]), 1); }
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&ctl->q_full[i]), 1);
-      mbar_init(smem_u32(&ctl->q_empty[i]), 1);
-      mbar_init(smem_u32(&ctl->s_full[i]), 1);
-      mbar_init(smem_u32(&ctl->p_ready[i]), 4);
+      mbar_init(smem_u32(&ctl->q_empty[i]), 2);
+      mbar_init(smem_u32(&ctl->s_full[i]), 2);
+      mbar_init(smem_u32(&ctl->s_read[i]), 4);
+      mbar_init(smem_u32(&ctl->p_ready[i][0]), 4);
+      mbar_init(smem_u32(&ctl->p_ready[i][1]), 4);
       mbar_init(smem_u32(&ctl->o_full[i]), 1);
       mbar_init(smem_u32(&ctl->o_free[i]), 4);
     }
@@ -493,7 +584,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&ctl->tmem_base);
+  const uint32_t tmem = uniform(*reinterpret_cast<volatile uint32_t*>(&ctl->tmem_base));
   follow_previous_kernel();
 
   if (warp < kWarpConvert) {
@@ -505,8 +596,9 @@ chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
   } else {
     setmaxnreg_dec<kOtherRegs>();
     if (warp == kWarpLoad) load_role<D>(p, ctl, &map_q, &map_k, &map_v, smem_u32(tiles));
-    else if (warp == kWarpMma) mma_role<D>(p, ctl, smem_u32(tiles), tmem);
-    else if (warp == kWarpWalk) walk_role<D>(p, ctl);
+    else if (warp == kWarpScore) score_role<D>(p, ctl, smem_u32(tiles), tmem);
+    else if (warp == kWarpOutput) output_role<D>(p, ctl, smem_u32(tiles), tmem);
+    else walk_role<D>(p, ctl);
   }
   __syncwarp();
   if (ctl->abort) {                                  // copies still in flight land before their memory is used again

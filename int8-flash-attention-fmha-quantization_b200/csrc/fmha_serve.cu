@@ -157,8 +157,12 @@ int fill_call(Call* c, const float amax[5], const int desc6[6], const void* q, c
     if (!(amax[i] > 0.f) || !std::isfinite(amax[i])) return FMHA_I8_ERR_BAD_AMAX;
   grouped::Params& p = c->p;
   const double c2 = static_cast<double>(amax[0]) * amax[1] / (127.0 * 127.0) / std::sqrt(static_cast<double>(D)) * 1.4426950408889634;
-  // between factors at which all probabilities are 1 and at which only the largest counts (the scores are integers up to 2^21)
-  p.c2 = static_cast<float>(std::min(std::max(c2, 0x1p-100), 64.0));
+  // Between factors at which all probabilities are 1 and at which only the largest counts (the scores are integers up to 2^21), rounded to 22 bits: half a
+  // step is 2^-23 of an exponent, of which fp16 sees 24 at the most.
+  int exponent;
+  const double mantissa = std::frexp(std::min(std::max(c2, 0x1p-100), 32.0), &exponent);
+  p.c2 = static_cast<float>(std::ldexp(std::nearbyint(std::ldexp(mantissa, 22)), exponent - 22));
+  p.growth = static_cast<int>(std::min(13.0 / p.c2, 1e9));
   p.out_scale = o_type == FMHA_I8_TYPE_I8 ? static_cast<float>(static_cast<double>(amax[2]) / amax[3]) : amax[2] / 127.f;
   if (!std::isfinite(p.out_scale)) return FMHA_I8_ERR_BAD_AMAX;
   p.q = static_cast<const int8_t*>(q);

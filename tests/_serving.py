@@ -45,16 +45,15 @@ def attention64(q, k, v, amax, causal):
 
 def tolerance(o, spread, keys, o_type, amax, o_amax):
     """Elementwise bound of |result - o|, o in real units.
-      P        fp16: half a step, 2^-11 relative, of every p: 2^-11 sum p |v|; below 2^-14 half a step is 2^-25 of the largest p (which is 2^-8 at the least
-               where the exponent's reference is kept while a row's maximum grows by less than 2^8, or is rounded): 2^-17 |v| per key, of sum p >= 1
-               times that, i.e. at most keys * 2^-25 / 2^-8 * v_amax where rows are that uneven; rows here are not: the sum of p is at
-               least the largest p, and 2^-25 * keys * v_amax is what is allowed.
-      exp2     2^-22, its argument (|a| <= 24 where p matters to fp16) rounded to 2^-24 relative: 24 * 2^-24 < 2^-19 together.
+      P        fp16: half a step, 2^-11 relative, of every p: 2^-11 sum p |v|; below 2^-14 half a step is 2^-25, absolute, where the row's largest p is 1 or
+               more, so that the sum of p is too: keys * 2^-25 * v_amax.
+      exp2     2^-22; its argument (|a| <= 24 where p matters to fp16) is off by half a step of the factor (22 bits: 2^-23 relative), of the factor's own
+               formula in fp32 (2^-24) and of its rounding (2^-24): 24 * 2^-22 * ln 2 < 2^-17.9; with the rest 2^-17.8 together.
       sums     keys additions in fp32, half a step (2^-24) each, of sums at most sum p |v|.
       output   half a step of its type relative to the result (int8: half a code)."""
     out = torch.full_like(o, 0.5 * o_amax / 127.0) if o_type == "int8" else o.abs() * (torch.finfo(TYPES[o_type]).eps / 2)
     tiny = 0.0 if o_type != "fp16" else 2.0 ** -25            # half a step below fp16's smallest normal number
-    return out * 1.001 + spread * (2.0 ** -11 + 2.0 ** -18 + keys * 2.0 ** -24) + keys * 2.0 ** -25 * amax[2] + tiny
+    return out * 1.001 + spread * (2.0 ** -11 + 2.0 ** -17.8 + keys * 2.0 ** -24) + keys * 2.0 ** -25 * amax[2] + tiny
 
 
 def real_units(o, o_type, o_amax):
