@@ -523,19 +523,17 @@ template <int D> __device__ __forceinline__ void softmax_role(const Params& p, C
       const float l = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       scale = l > 0.f ? p.out_scale / l : 0.f;
     }
-    const bool some = limit > 0;
+    if (limit <= 0) scale = 0.f;
 #pragma unroll 1
     for (int i = 0; i < D; i += 32) {
       uint32_t o[32];
       if (n > 0 && any) tmem_ld32(tO + i, o);
       if (real) {
+        if (limit <= 0) {                            // (what stands in its place may be no number)
 #pragma unroll
-        for (int x = 0; x < 32; x += 4) {
-          float v[4];
-#pragma unroll
-          for (int y = 0; y < 4; ++y) v[y] = some ? __uint_as_float(o[x + y]) * scale : 0.f;
-          store4(p.o, p.o_type, at + i + x, v);
+          for (int x = 0; x < 32; ++x) o[x] = 0u;
         }
+        store32(p.o, p.o_type, p.o_wide != 0, at + i, o, scale);
       }
       __syncwarp();
     }

@@ -37,6 +37,7 @@ struct Params {
   int B, H, Hkv, G;
   int total_q, total_k, max_q;
   int o_type, causal;
+  int o_wide;                          // rows of o are 32-byte aligned
   int row_groups;                      // rows kernel: groups of 16 rows per sequence and key head
   int tq;                              // chunk kernel: tokens per tile of 128 rows
   float c2;                            // from a difference of scores to an exponent of 2; 22 bits, so that 3 c2 is exact
@@ -145,6 +146,46 @@ __device__ __forceinline__ void store4(void* o, int type, long long at, const fl
   } else {
     __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
     *reinterpret_cast<uint2*>(static_cast<__half*>(o) + at) = make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
+  }
+}
+
+// Thirty-two neighbouring outputs x * scale, x as the bits of floats.  A warp's threads write rows of their own, so that every store instruction touches 32 lines
+// whatever its width; `wide`: rows are 32-byte aligned, and fewer and wider stores will do.
+__device__ __forceinline__ void store32(void* o, int type, bool wide, long long at, const uint32_t (&x)[32], float scale) {
+  uint32_t w[16];
+  auto value = [&](int i) { return __uint_as_float(x[i]) * scale; };
+  if (type == FMHA_I8_TYPE_I8) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float v[4];
+#pragma unroll
+      for (int y = 0; y < 4; ++y) v[y] = fminf(fmaxf(value(4 * i + y), -127.f), 127.f) + kMagic;
+      w[i] = __byte_perm(__byte_perm(__float_as_uint(v[0]), __float_as_uint(v[1]), 0x0040), __byte_perm(__float_as_uint(v[2]), __float_as_uint(v[3]), 0x0040), 0x5410);
+    }
+  } else if (type == FMHA_I8_TYPE_BF16) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(value(2 * i), value(2 * i + 1));
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const __half2 h = __floats2half2_rn(value(2 * i), value(2 * i + 1));
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+  uint8_t* to = static_cast<uint8_t*>(o) + at * (type == FMHA_I8_TYPE_I8 ? 1 : 2);
+  const int words = type == FMHA_I8_TYPE_I8 ? 8 : 16;
+#pragma unroll
+  for (int i = 0; i < 16; i += 8) {
+    if (i >= words) break;
+    if (wide) {
+      st_global_v8(to + 4 * i, reinterpret_cast<const uint32_t(&)[8]>(w[i]));
+    } else {
+      *reinterpret_cast<uint4*>(to + 4 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+      *reinterpret_cast<uint4*>(to + 4 * i + 16) = make_uint4(w[i + 4], w[i + 5], w[i + 6], w[i + 7]);
+    }
   }
 }
 

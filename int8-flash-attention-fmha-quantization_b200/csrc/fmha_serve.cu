@@ -174,6 +174,7 @@ int fill_call(Call* c, const float amax[5], const int desc6[6], const void* q, c
   p.total_q = static_cast<int>(total_q);
   p.max_q = max_q;
   p.o_type = o_type;
+  p.o_wide = aligned(o, 32) && o_stride * type_bytes(o_type) % 32 == 0;
   p.causal = (flags & FMHA_I8_FLAG_CAUSAL) != 0u;
   c->k = k;
   c->v = v;
