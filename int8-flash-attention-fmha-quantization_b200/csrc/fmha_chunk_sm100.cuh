@@ -31,16 +31,17 @@ constexpr int kWarpConvert = 8, kWarpLoad = 12, kWarpScore = 13, kWarpWalk = 14,
 constexpr int kInfos = 4;
 constexpr int kInfoConsumers = 8 + 4 + 1 + 2;      // softmax warps, converters, loader, issuers
 constexpr uint32_t kTmemCols = 512;
-constexpr int kLowest = -(1 << 22);                                      // below every score (127 * 127 * 128 < 2^21)
-// A score that, with kMagicBits and less any other score, is the bits of a float of about -2^127, whose exponential is zero.
-constexpr int kMasked = static_cast<int>(0xFF000000u - kMagicBits);
+// Scores come as the bits of the float kMagic + score (see issue_scores), which order like integers.
+constexpr int kLowest = static_cast<int>(kMagicBits) - (1 << 22);        // below every score (127 * 127 * 128 < 2^21)
+constexpr uint32_t kMasked = 0xFF000000u;                                // -2^127: below that, and its exponential is zero
 
 template <int D> struct Cfg {
   static constexpr int kTileBytes = kTile * D;
   static constexpr int kStagesK = 3, kStagesV = 2, kStagesH = 2;          // K, V as int8, V as fp16
   static constexpr int kHalfBytes = 2 * kTileBytes;                      // a tile of V as fp16
   static constexpr int kQ = 0, kK = 4 * kTileBytes, kV = kK + kStagesK * kTileBytes, kH = kV + kStagesV * kTileBytes;
-  static constexpr int kBytes = kH + kStagesH * kHalfBytes;
+  static constexpr int kBias = kH + kStagesH * kHalfBytes;              // constant operands, 128 and 64 rows of 32 bytes
+  static constexpr int kBytes = kBias + (kTile + kTile / 2) * 32;
 };
 // What all roles need to know of a unit, and what the loader and the softmax warps do.
 struct Steps {
@@ -282,10 +283,13 @@ template <int D> __device__ __forceinline__ void convert_role(const Params& p, C
 // cycles for a step of one tile, of which the tensor core is busy 450).
 // P of a step takes the first half of the columns of its scores.  The scores of the next step's last 64 keys therefore follow as soon as these are in
 // registers (one warp), those of the first 64 behind the P.V that reads P (the other: MMAs of one thread execute in order).
-template <int D> __device__ __forceinline__ void issue_scores(uint32_t dst, uint64_t dq, uint64_t dk) {
+// S of 64 keys.  The accumulator is first set to 2048 * 6144 = kMagic by a product of constants (16 bits, one step); the integer products then add to the
+// bits of that float, which reads as kMagic + score without a conversion: 128 integer additions of a thread less, 8 % of a long prompt.
+template <int D> __device__ __forceinline__ void issue_scores(uint32_t dst, uint64_t dq, uint64_t dk, uint32_t bias) {
   constexpr uint32_t kIdescS = make_idesc_i8(kTile / 2, false);
+  mma_f16_ss(dst, make_smem_desc_noswizzle(bias, 128, 256), make_smem_desc_noswizzle(bias + kTile * 32, 128, 256), make_idesc_bf16(kTile / 2), 0);
 #pragma unroll
-  for (int y = 0; y < D / 32; ++y) mma_i8_ss(dst, desc_advance(dq, 32 * y), desc_advance(dk, 32 * y), kIdescS, y > 0);
+  for (int y = 0; y < D / 32; ++y) mma_i8_ss(dst, desc_advance(dq, 32 * y), desc_advance(dk, 32 * y), kIdescS, 1);
 }
 template <int D> __device__ __forceinline__ void score_role(const Params& p, Ctl<D>* ctl, uint32_t smem, uint32_t tmem) {
   using C = Cfg<D>;
@@ -314,7 +318,7 @@ template <int D> __device__ __forceinline__ void score_role(const Params& p, Ctl
         if (c > 0 && !warp_wait(smem_u32(&ctl->s_read[t]), (c - 1) & 1u, abort_flag)) return fail(FMHA_I8_DEV_WAIT_S_FREE, c);
         tc_fence_after();
         if (elect_one()) {
-          issue_scores<D>(tmem + t * kTile + kTile / 2, make_smem_desc(smem + C::kQ + (2 * q + t) * C::kTileBytes, D), dk);
+          issue_scores<D>(tmem + t * kTile + kTile / 2, make_smem_desc(smem + C::kQ + (2 * q + t) * C::kTileBytes, D), dk, smem + C::kBias);
           mma_commit(smem_u32(&ctl->s_full[t]));
         }
         __syncwarp();
@@ -379,7 +383,7 @@ template <int D> __device__ __forceinline__ void output_role(const Params& p, Ct
         if (i + 1 < n) {
           tc_fence_after();
           if (elect_one()) {
-            issue_scores<D>(tmem + t * kTile, make_smem_desc(smem + C::kQ + (2 * q + t) * C::kTileBytes, D), dk);
+            issue_scores<D>(tmem + t * kTile, make_smem_desc(smem + C::kQ + (2 * q + t) * C::kTileBytes, D), dk, smem + C::kBias);
             mma_commit(smem_u32(&ctl->s_full[t]));
           }
           __syncwarp();
@@ -404,7 +408,7 @@ template <int D> __device__ __forceinline__ void output_role(const Params& p, Ct
 // ------------------------------------------------------------------------------------------------ softmax
 __device__ __forceinline__ int max3(int a, int b, int c) { return __vimax3_s32(a, b, c); }
 
-template <int D> __device__ __forceinline__ void softmax_role(const Params& p, Ctl<D>* ctl, uint32_t tmem) {
+template <int D, bool kWide> __device__ __forceinline__ void softmax_role(const Params& p, Ctl<D>* ctl, uint32_t tmem) {
   const int warp = warp_index(), t = warp >> 2, quad = warp & 3, lane = threadIdx.x & 31;
   const int row = quad * 32 + lane;
   const Failure fail{p, &ctl->abort};
@@ -412,7 +416,7 @@ template <int D> __device__ __forceinline__ void softmax_role(const Params& p, C
   const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
   const uint32_t tS = tmem + lanes + t * kTile, tO = tmem + lanes + 2 * kTile + t * kTile;
   const int my_token = row / p.G;
-  const float2 c2 = make_float2(p.c2, p.c2), less = make_float2(-kMagic * p.c2, -kMagic * p.c2);
+  const float2 c2 = make_float2(p.c2, p.c2);
   UnitReader<D> units{ctl};
   uint32_t steps = 0, outs = 0;
   while (true) {
@@ -429,14 +433,17 @@ template <int D> __device__ __forceinline__ void softmax_role(const Params& p, C
     }
     const bool any = __any_sync(0xFFFFFFFFu, limit > 0);            // a warp without a row that sees a key leaves its part of P as it is
     const int least = __reduce_min_sync(0xFFFFFFFFu, real ? limit : 0x7FFFFFFF);
-    // p = 2^((s - ref) c2), with an integer ref.  kMagicBits + (s - ref) are the bits of the float kMagic + (s - ref), exactly, and c2 has so few of them that
-    // kMagic * c2 is a float too: one multiply-add gives the exponent, rounded once.
+    // p = 2^((x - ref) c2), x and ref as the floats kMagic + score.  Exponents are x c2 - hi with hi = ref c2 rounded, the same for a row as long as its
+    // reference is, and rounded once.  Where c2 is large the difference is taken first: hi would be off by as much as 16.
     int ref = 0;
+    float hi = 0.f;
     float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll 1
     for (int i = 0; i < n; ++i, ++steps) {
       if (!warp_wait(smem_u32(&ctl->s_full[t]), steps & 1u, abort_flag)) return fail(FMHA_I8_DEV_WAIT_S_READY, steps);
       uint32_t r[8][16];
+      bool grew = false;
+      float factor = 1.f;
       if (any) {
         tc_fence_after();
 #pragma unroll
@@ -452,7 +459,7 @@ template <int D> __device__ __forceinline__ void softmax_role(const Params& p, C
           const int open = limit - i * kTile;
 #pragma unroll
           for (int x = 0; x < kTile; ++x)
-            if (x >= open) r[x >> 4][x & 15] = static_cast<uint32_t>(kMasked);
+            if (x >= open) r[x >> 4][x & 15] = kMasked;
         }
         int m0 = kLowest, m1 = kLowest;
 #pragma unroll
@@ -463,34 +470,44 @@ template <int D> __device__ __forceinline__ void softmax_role(const Params& p, C
         const int m = max(m0, m1);
         if (i == 0) {
           ref = m;
+          hi = __int_as_float(m) * p.c2;
         } else {
           const bool grown = m - ref > p.growth;
           if (__any_sync(0xFFFFFFFFu, grown)) {
-            const float factor = grown ? ex2(static_cast<float>(ref - m) * p.c2) : 1.f;
+            grew = true;
+            const float next = grown ? __int_as_float(m) * p.c2 : hi;
+            factor = !grown ? 1.f : kWide ? ex2((__int_as_float(ref) - __int_as_float(m)) * p.c2) : ex2(hi - next);
             if (grown) ref = m;
+            hi = next;
             sum[0].x *= factor; sum[0].y *= factor; sum[1].x *= factor; sum[1].y *= factor;
-            // (the scores that have just been read were formed behind P.V of the step before)
-#pragma unroll 1
-            for (int x = 0; x < D; x += 16) {
-              uint32_t o[16];
-              tmem_ld16_issue(tO + x, o);
-              tmem_ld_fence(o);
-#pragma unroll
-              for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * factor);
-              tmem_st16(tO + x, o);
-            }
           }
         }
       }
       if (any) {
-        const uint32_t bits = kMagicBits - static_cast<uint32_t>(ref);
+        const float2 less = make_float2(-hi, -hi), from = make_float2(-__int_as_float(ref), -__int_as_float(ref));
 #pragma unroll
         for (int h = 0; h < 8; ++h) {
+          if (h == 4 && grew) {
+            // The reference has moved: what has been summed so far is rescaled before more is added.  (The scores of this step were formed behind P.V of the one
+            // before.)  Here, where half of the scores have become powers, there are registers for 32 columns at a time.
+#pragma unroll 1
+            for (int x = 0; x < D; x += 16) {
+              uint32_t o[1][16];
+              tmem_ld16_issue(tO + x, o[0]);
+#pragma unroll
+              for (int z = 0; z < 1; ++z) {
+                tmem_ld_fence(o[z]);
+#pragma unroll
+                for (int y = 0; y < 16; ++y) o[z][y] = __float_as_uint(__uint_as_float(o[z][y]) * factor);
+                tmem_st16(tO + x + 16 * z, o[z]);
+              }
+            }
+          }
           uint32_t packed[8];
 #pragma unroll
           for (int x = 0; x < 8; ++x) {
-            const float2 v = make_float2(__uint_as_float(r[h][2 * x] + bits), __uint_as_float(r[h][2 * x + 1] + bits));
-            const float2 a = __ffma2_rn(v, c2, less);
+            const float2 v = make_float2(__uint_as_float(r[h][2 * x]), __uint_as_float(r[h][2 * x + 1]));
+            const float2 a = kWide ? __fmul2_rn(__fadd2_rn(v, from), c2) : __ffma2_rn(v, c2, less);
             const float2 e = make_float2(ex2(a.x), ex2(a.y));
             sum[x & 1] = __fadd2_rn(sum[x & 1], e);
             const __half2 q = __floats2half2_rn(e.x, e.y);
@@ -545,7 +562,8 @@ template <int D> __device__ __forceinline__ void softmax_role(const Params& p, C
   }
 }
 
-template <int D>
+// kWide: the factor from scores to exponents is large (see softmax_role).
+template <int D, bool kWide>
 __global__ void __launch_bounds__(kThreads, 1)
 chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Params p) {
   using C = Cfg<D>;
@@ -579,6 +597,9 @@ chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     tmem_alloc(smem_u32(&ctl->tmem_base), kTmemCols);
     tmem_relinquish();
   }
+  for (int i = threadIdx.x; i < (kTile + kTile / 2) * 2; i += kThreads)      // unswizzled: 8 rows of 16 bytes, the other half of their K behind them
+    reinterpret_cast<uint4*>(tiles + C::kBias)[i] = make_uint4((i & 8) ? 0u : i < kTile * 2 ? 0x4500u : 0x45C0u, 0u, 0u, 0u);      // 2048 and 6144 in bf16
+  fence_proxy_async_smem();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -587,7 +608,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
 
   if (warp < kWarpConvert) {
     setmaxnreg_inc<kSoftmaxRegs>();
-    softmax_role<D>(p, ctl, tmem);
+    softmax_role<D, kWide>(p, ctl, tmem);
   } else if (warp < kWarpLoad) {
     setmaxnreg_dec<kConvertRegs>();
     convert_role<D>(p, ctl, tiles);

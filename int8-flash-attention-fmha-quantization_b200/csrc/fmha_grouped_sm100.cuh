@@ -40,8 +40,8 @@ struct Params {
   int o_wide;                          // rows of o are 32-byte aligned
   int row_groups;                      // rows kernel: groups of 16 rows per sequence and key head
   int tq;                              // chunk kernel: tokens per tile of 128 rows
-  float c2;                            // from a difference of scores to an exponent of 2; 22 bits, so that 3 c2 is exact
-  int growth;                          // chunk kernel: a reference is kept while the maximum exceeds it by no more than this, 2^13 in p
+  float c2;                            // from a difference of scores to an exponent of 2
+  int growth;                          // chunk kernel: a reference is kept while the maximum exceeds it by no more than this, 2^14 in p
   float out_scale;                     // from sum p v / sum p, v in codes, to the output's unit
   unsigned* status;                    // eight device status words
   unsigned* host_word;                 // the host-visible failure word

@@ -90,17 +90,19 @@ template <int D> int set_up_rows(int* clusters16) {
 }
 
 template <int D> int set_up_chunk() {
-  const void* fn = reinterpret_cast<const void*>(&chunk::chunk_kernel<D>);
-  cudaFuncAttributes fa{};
-  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(chunk::smem_bytes<D>())) != cudaSuccess ||
-      cudaFuncGetAttributes(&fa, fn) != cudaSuccess) {
-    cudaGetLastError();
+  for (const void* fn : {reinterpret_cast<const void*>(&chunk::chunk_kernel<D, false>), reinterpret_cast<const void*>(&chunk::chunk_kernel<D, true>)}) {
+    cudaFuncAttributes fa{};
+    if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(chunk::smem_bytes<D>())) != cudaSuccess ||
+        cudaFuncGetAttributes(&fa, fn) != cudaSuccess) {
+      cudaGetLastError();
+      return FMHA_I8_ERR_LAUNCH;
+    }
+    // the kernel moves registers between its warps with setmaxnreg, which only terminates if the launch allocation is what the targets were sized for
+    if (fa.numRegs == chunk::kLaunchRegs) continue;
+    std::fprintf(stderr, "fmha_i8_sm100: chunk kernel built with %d registers per thread, expected %d; refusing to launch\n", fa.numRegs, chunk::kLaunchRegs);
     return FMHA_I8_ERR_LAUNCH;
   }
-  // the kernel moves registers between its warps with setmaxnreg, which only terminates if the launch allocation is what the targets were sized for
-  if (fa.numRegs == chunk::kLaunchRegs) return FMHA_I8_OK;
-  std::fprintf(stderr, "fmha_i8_sm100: chunk kernel built with %d registers per thread, expected %d; refusing to launch\n", fa.numRegs, chunk::kLaunchRegs);
-  return FMHA_I8_ERR_LAUNCH;
+  return FMHA_I8_OK;
 }
 
 int set_up(const Device& dev) {
@@ -157,12 +159,9 @@ int fill_call(Call* c, const float amax[5], const int desc6[6], const void* q, c
     if (!(amax[i] > 0.f) || !std::isfinite(amax[i])) return FMHA_I8_ERR_BAD_AMAX;
   grouped::Params& p = c->p;
   const double c2 = static_cast<double>(amax[0]) * amax[1] / (127.0 * 127.0) / std::sqrt(static_cast<double>(D)) * 1.4426950408889634;
-  // Between factors at which all probabilities are 1 and at which only the largest counts (the scores are integers up to 2^21), rounded to 22 bits: half a
-  // step is 2^-23 of an exponent, of which fp16 sees 24 at the most.
-  int exponent;
-  const double mantissa = std::frexp(std::min(std::max(c2, 0x1p-100), 32.0), &exponent);
-  p.c2 = static_cast<float>(std::ldexp(std::nearbyint(std::ldexp(mantissa, 22)), exponent - 22));
-  p.growth = static_cast<int>(std::min(13.0 / p.c2, 1e9));
+  // between factors at which all probabilities are 1 and at which only the largest counts (the scores are integers up to 2^21)
+  p.c2 = static_cast<float>(std::min(std::max(c2, 0x1p-100), 32.0));
+  p.growth = static_cast<int>(std::min(14.0 / p.c2, 1e9));
   p.out_scale = o_type == FMHA_I8_TYPE_I8 ? static_cast<float>(static_cast<double>(amax[2]) / amax[3]) : amax[2] / 127.f;
   if (!std::isfinite(p.out_scale)) return FMHA_I8_ERR_BAD_AMAX;
   p.q = static_cast<const int8_t*>(q);
@@ -218,7 +217,7 @@ template <int D> int launch_chunk(cudaStream_t stream, const Device& dev, Call& 
   const long long units = std::min<long long>(p.total_q, p.total_q / (2LL * p.tq) + p.B) * p.Hkv;
   if (units > kMostRows) return FMHA_I8_ERR_TOO_LARGE;
   const unsigned grid = static_cast<unsigned>(std::min<long long>(units, dev.sm_count));
-  return launch(chunk::chunk_kernel<D>, grid, chunk::kThreads, chunk::smem_bytes<D>(), stream, 0u, mq, mk, mv, p);
+  return launch(p.c2 > 0.5f ? chunk::chunk_kernel<D, true> : chunk::chunk_kernel<D, false>, grid, chunk::kThreads, chunk::smem_bytes<D>(), stream, 0u, mq, mk, mv, p);
 }
 
 int run_attention(void* stream, Call& c) {
