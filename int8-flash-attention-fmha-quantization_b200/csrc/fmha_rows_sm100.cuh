@@ -3,13 +3,17 @@
 //
 // The G heads of a group and the new tokens of a sequence make the rows: row r is token r / G, head r % G of the group, sixteen at a time.
 // What bounds it: K and V of a key head are read once for all of a group's rows, so HBM does, 2 D bytes per key.  A tensor-core tile of
-// tcgen05.mma has 128 rows; here sixteen are enough, so the products are warp-level ones (m16n8k16, fp16 in, fp32 out), and
+// tcgen05.mma has 128 rows; here eight or sixteen are enough, so the products are warp-level ones, and
 //   * a warp owns whole tiles of 128 keys, with its running maximum, sum and output rows in registers; it asks for its next K
 //     when it has formed the scores of this one, and for the next V behind P.V;
-//   * int8 becomes fp16 in registers on its way from shared memory into the product: integers up to 2048 are exact there, and the
-//     scores are exact in fp32 (at most 127 * 127 * 128 < 2^24).  Which key, column or row a lane's element belongs to is free as
-//     long as both operands agree, and is chosen so that each lane reads 16 bytes at a time without bank conflicts from the swizzled
-//     tiles, and so that the scores' registers are P's operand as they are;
+//   * scores are products of bytes (m16n8k32) on top of the bits of the float kMagic, so that they read as kMagic + score;
+//   * up to eight rows (one token of a model with up to eight query heads to a key head), P is a whole number of 16 bits, rn(65535 p) with p relative to the
+//     running maximum: its upper bytes make rows 0-7 of the product with V, its lower bytes rows 8-15.  Nothing is converted and no row is idle; the sums
+//     are exact and stay whole numbers until the maximum of a row grows.  2^-17 of the largest p for every key; fp16's 2^-12 of each p is no better where
+//     a row spreads over many keys, and 2900 instructions a tile became 800;
+//   * up to sixteen rows P is fp16 and V becomes fp16 in registers (integers up to 2048 are exact there), m16n8k16;
+//   * which key, column or row a lane's element belongs to is free as long as both operands agree, and is chosen so that each lane reads 16 bytes at a time
+//     without bank conflicts from the swizzled tiles, and so that the scores' registers are P's operand as they are;
 //   * the keys of a sequence are split over the warps of a cluster of CTAs, whose partial rows meet through distributed shared memory.
 #pragma once
 #include "fmha_grouped_sm100.cuh"
@@ -19,15 +23,16 @@ namespace rows {
 
 using namespace grouped;
 
-constexpr int kRows = 16;
 constexpr int kMaxCluster = 16;
+constexpr float kLevels = 65535.f;                   // of P in 16 bits
+constexpr int kFlushTiles = 512;                     // 65,536 keys * 127 * 255 < 2^31
 // 64 KB of tiles per CTA and three CTAs to an SM, or one CTA with three times as many warps
 template <int D> struct Cfg {
   static constexpr int kWarps = (D == 128) ? 2 : 4;
   static constexpr int kWarpsWide = 3 * kWarps;
   static constexpr int kTileBytes = kTile * D;
 };
-template <int D, int W> struct Smem {
+template <int D, int W, int kRows> struct Smem {
   alignas(1024) uint8_t ring[2 * W * kTile * D];     // per warp: one K tile, one V tile; at the end its partial rows
   float2 stat[W][kRows];                             // reference exponent and sum of each partial row
   float weight[kMaxCluster * W][kRows];              // what each partial row counts in the whole
@@ -38,6 +43,17 @@ template <int D, int W> struct Smem {
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16832(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// A unsigned
+__device__ __forceinline__ void mma16832_u(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint4 lds16(uint32_t at) {
@@ -56,15 +72,17 @@ template <int D> __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
   return D == 128 ? static_cast<uint32_t>(r * 128 + ((c ^ (r & 7)) << 4)) : static_cast<uint32_t>(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
 }
 
-// grid: clusters of c CTAs, one per (sequence, key head, group of rows).
-template <int D, int W>
+// grid: clusters of c CTAs, one per (sequence, key head, group of kRows rows).  kRows: 8 or 16.
+template <int D, int W, int kRows>
 __global__ void __launch_bounds__(W * 32, W <= 4 ? 3 : 1)
 rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Params p) {
   using C = Cfg<D>;
-  constexpr int kSteps = D / 16;                     // products of 16 columns in a score; 8-column tiles of the output are D / 8
-  constexpr int kOut = D / 8;
+  constexpr bool kEight = kRows == 8;
+  constexpr int kHalves = kRows / 8;                 // rows of a lane
+  constexpr int kWords = D / 16;                     // words that a lane holds of a row of Q or K
+  constexpr int kOut = D / 8;                        // 8-column tiles of the output
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  Smem<D, W>& sm = *reinterpret_cast<Smem<D, W>*>(smem_raw);
+  Smem<D, W, kRows>& sm = *reinterpret_cast<Smem<D, W, kRows>*>(smem_raw);
   const int lane = threadIdx.x & 31, warp = warp_index();
   const int ctas = static_cast<int>(cluster_ctas()), rank = static_cast<int>(cluster_rank());
   if (threadIdx.x == 0) sm.abort = 0;
@@ -87,27 +105,25 @@ rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
   if (row0 >= n_rows) return;                        // the whole cluster
   const int end = visible(p, s, min(row0 + kRows - 1, n_rows - 1) / p.G);      // the last token of the group sees most
   const int n_tiles = (end + kTile - 1) / kTile;
-  const int first = n_tiles * rank / ctas, last = n_tiles * (rank + 1) / ctas; // this CTA's share
+  const int first = static_cast<int>(static_cast<long long>(n_tiles) * rank / ctas), last = static_cast<int>(static_cast<long long>(n_tiles) * (rank + 1) / ctas);
 
-  const int g = lane >> 2, t4 = lane & 3;            // my rows: g and g + 8
-  uint32_t qa[kSteps][4];
-  int limit[2];
+  const int g = lane >> 2, t4 = lane & 3;            // my rows: g, and g + 8 of sixteen
+  uint32_t qa[kHalves][kWords];
+  int limit[kHalves], least = 0x7FFFFFFF;            // keys that my rows see, that all rows see
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+  for (int h = 0; h < kHalves; ++h) {
     const int row = row0 + g + 8 * h, token = row / p.G;
     const bool real = row < n_rows;
     limit[h] = real ? visible(p, s, token) : 0;
+    least = min(least, limit[h]);
     const uint4* src = reinterpret_cast<const uint4*>(p.q + (s.q0 + token) * p.q_stride + (head * p.G + row - token * p.G) * D + t4 * (D / 4));
 #pragma unroll
     for (int c = 0; c < D / 64; ++c) {
       const uint4 w = real ? src[c] : make_uint4(0u, 0u, 0u, 0u);
-      unpack4(w.x, qa[4 * c][h], qa[4 * c][2 + h]);
-      unpack4(w.y, qa[4 * c + 1][h], qa[4 * c + 1][2 + h]);
-      unpack4(w.z, qa[4 * c + 2][h], qa[4 * c + 2][2 + h]);
-      unpack4(w.w, qa[4 * c + 3][h], qa[4 * c + 3][2 + h]);
+      qa[h][4 * c] = w.x; qa[h][4 * c + 1] = w.y; qa[h][4 * c + 2] = w.z; qa[h][4 * c + 3] = w.w;
     }
   }
-  const int least = __reduce_min_sync(0xFFFFFFFFu, min(limit[0], limit[1]));   // keys that all rows see
+  least = __reduce_min_sync(0xFFFFFFFFu, least);
 
   const uint32_t k_tile = smem_u32(sm.ring) + static_cast<uint32_t>(warp * 2 * C::kTileBytes), v_tile = k_tile + C::kTileBytes;
   const uint32_t bar_k = smem_u32(&sm.k_full[warp]), bar_v = smem_u32(&sm.v_full[warp]);
@@ -121,11 +137,29 @@ rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
     if (lane < n) issue_copy<D>(p, map, dst, bar, s, head, tile * kTile, lane, page);
   };
 
-  float o[kOut][4], ref[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};      // p = 2^(s c2 - ref)
+  // Outputs: rows g (and g + 8) times columns n = 2 t4 and 2 t4 + 1 of kOut tiles.  Of eight rows, `whole` has the sums since the last change of a reference,
+  // of the upper bytes of P in [0], [1] and of the lower ones in [2], [3].
+  float o[kHalves][kOut][2], ref[kHalves], sum[kHalves];      // p = 2^((x - ref) c2)
+  int whole[kEight ? kOut : 1][4];
+  int held = 0;                                      // tiles in `whole`
 #pragma unroll
-  for (int j = 0; j < kOut; ++j)
+  for (int h = 0; h < kHalves; ++h) {
+    ref[h] = -INFINITY;
+    sum[h] = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[j][i] = 0.f;
+    for (int j = 0; j < kOut; ++j) o[h][j][0] = o[h][j][1] = 0.f;
+  }
+#pragma unroll
+  for (int j = 0; j < (kEight ? kOut : 1); ++j) whole[j][0] = whole[j][1] = whole[j][2] = whole[j][3] = 0;
+  auto flush = [&](float shrink) {
+#pragma unroll
+    for (int j = 0; j < (kEight ? kOut : 1); ++j) {
+      o[0][j][0] = (o[0][j][0] + fmaf(256.f, static_cast<float>(whole[j][0]), static_cast<float>(whole[j][2]))) * shrink;
+      o[0][j][1] = (o[0][j][1] + fmaf(256.f, static_cast<float>(whole[j][1]), static_cast<float>(whole[j][3]))) * shrink;
+      whole[j][0] = whole[j][1] = whole[j][2] = whole[j][3] = 0;
+    }
+    held = 0;
+  };
 
   bool ok = true;
   uint32_t n = 0;
@@ -140,23 +174,20 @@ rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
     if (more) next_page = page_of(p, b, (tile + W) * kTile, end, lane);
     // ---- scores: column n of product j is key 8 j + n; my columns of K are the D / 4 from t4 * D / 4 on
     if (!(ok = __all_sync(0xFFFFFFFFu, mbar_wait_timed(bar_k, n & 1u, abort_flag)))) break;
-    float sc[16][4];
+    float x[kHalves][16][2];
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
+      int c[4] = {static_cast<int>(kMagicBits), static_cast<int>(kMagicBits), static_cast<int>(kMagicBits), static_cast<int>(kMagicBits)};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sc[j][i] = 0.f;
+      for (int y = 0; y < D / 64; ++y) {
+        const uint4 w = lds16(k_tile + chunk_at<D>(8 * j + g, t4 * (D / 64) + y));
+        mma16832(c, qa[0][4 * y], kEight ? 0u : qa[kHalves - 1][4 * y], qa[0][4 * y + 1], kEight ? 0u : qa[kHalves - 1][4 * y + 1], w.x, w.y);
+        mma16832(c, qa[0][4 * y + 2], kEight ? 0u : qa[kHalves - 1][4 * y + 2], qa[0][4 * y + 3], kEight ? 0u : qa[kHalves - 1][4 * y + 3], w.z, w.w);
+      }
 #pragma unroll
-      for (int c = 0; c < D / 64; ++c) {
-        const uint4 w = lds16(k_tile + chunk_at<D>(8 * j + g, t4 * (D / 64) + c));
-        uint32_t lo, hi;
-        unpack4(w.x, lo, hi);
-        mma16816(sc[j], qa[4 * c][0], qa[4 * c][1], qa[4 * c][2], qa[4 * c][3], lo, hi);
-        unpack4(w.y, lo, hi);
-        mma16816(sc[j], qa[4 * c + 1][0], qa[4 * c + 1][1], qa[4 * c + 1][2], qa[4 * c + 1][3], lo, hi);
-        unpack4(w.z, lo, hi);
-        mma16816(sc[j], qa[4 * c + 2][0], qa[4 * c + 2][1], qa[4 * c + 2][2], qa[4 * c + 2][3], lo, hi);
-        unpack4(w.w, lo, hi);
-        mma16816(sc[j], qa[4 * c + 3][0], qa[4 * c + 3][1], qa[4 * c + 3][2], qa[4 * c + 3][3], lo, hi);
+      for (int h = 0; h < kHalves; ++h) {
+        x[h][j][0] = __int_as_float(c[2 * h]);
+        x[h][j][1] = __int_as_float(c[2 * h + 1]);
       }
     }
     __syncwarp();
@@ -164,65 +195,123 @@ rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
 
     if (tile * kTile + kTile > least) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
+      for (int h = 0; h < kHalves; ++h)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (tile * kTile + 8 * j + 2 * t4 + (i & 1) >= limit[i >> 1]) sc[j][i] = -INFINITY;
+        for (int j = 0; j < 16; ++j)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if (tile * kTile + 8 * j + 2 * t4 + i >= limit[h]) x[h][j][i] = -INFINITY;
     }
     // ---- softmax of the tile; lanes with the same g share rows
-    uint32_t pa[16][2];
+    float shrink[kHalves];
+    bool moved = false;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < kHalves; ++h) {
       float m = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) m = fmaxf(m, fmaxf(sc[j][2 * h], sc[j][2 * h + 1]));
+      for (int j = 0; j < 16; ++j) m = fmaxf(m, fmaxf(x[h][j][0], x[h][j][1]));
       m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
       m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
-      const float next = fmaxf(ref[h], m * p.c2);                    // the same float in every lane of the row
-      const float base = next == -INFINITY ? 0.f : next;             // a row that has seen no key yet: all p are zero
-      const float shrink = ex2(ref[h] - base);
+      const float next = fmaxf(ref[h], m);
+      moved |= next != ref[h];
+      shrink[h] = next == ref[h] ? 1.f : ex2((ref[h] - next) * p.c2);
       ref[h] = next;
-      float part = 0.f;
+    }
+    if (__any_sync(0xFFFFFFFFu, moved)) {
+      if constexpr (kEight) {
+        flush(shrink[0]);
+      } else {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const float p0 = ex2(fmaf(sc[j][2 * h], p.c2, -base)), p1 = ex2(fmaf(sc[j][2 * h + 1], p.c2, -base));
-        part += p0 + p1;
-        const __half2 packed = __floats2half2_rn(p0, p1);
-        pa[j][h] = *reinterpret_cast<const uint32_t*>(&packed);
-      }
-      sum[h] = fmaf(sum[h], shrink, part);
+        for (int h = 0; h < kHalves; ++h)
 #pragma unroll
-      for (int j = 0; j < kOut; ++j) {
-        o[j][2 * h] *= shrink;
-        o[j][2 * h + 1] *= shrink;
+          for (int j = 0; j < kOut; ++j) {
+            o[h][j][0] *= shrink[h];
+            o[h][j][1] *= shrink[h];
+          }
       }
     }
-
-    // ---- P.V: sixteen keys at a time; column n of output tile j is column n * D / 8 + j of V
-    if (!(ok = __all_sync(0xFFFFFFFFu, mbar_wait_timed(bar_v, n & 1u, abort_flag)))) break;
+    uint32_t pa[kHalves][16];                        // sixteen rows: two fp16 a tile of eight keys; eight rows: the 16-bit numbers of two keys
+    const float2 c2 = make_float2(p.c2, p.c2);
 #pragma unroll
-    for (int kb = 0; kb < 8; ++kb) {
-      uint32_t v[4][D / 32];                         // my D / 8 columns of four keys
+    for (int h = 0; h < kHalves; ++h) {
+      const float base = ref[h] == -INFINITY ? 0.f : ref[h];         // a row that has seen no key yet: all p are zero
+      float2 part = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int key = 16 * kb + 2 * t4 + (r & 1) + 8 * (r >> 1);
-        if constexpr (D == 128) {
-          const uint4 w = lds16(v_tile + chunk_at<D>(key, g));
-          v[r][0] = w.x; v[r][1] = w.y; v[r][2] = w.z; v[r][3] = w.w;
+      for (int j = 0; j < 16; ++j) {
+        const float2 a = __fmul2_rn(__fadd2_rn(make_float2(x[h][j][0], x[h][j][1]), make_float2(-base, -base)), c2);
+        const float2 e = make_float2(ex2(a.x), ex2(a.y));
+        part = __fadd2_rn(part, e);
+        if constexpr (kEight) {
+          const float2 y = __ffma2_rn(e, make_float2(kLevels, kLevels), make_float2(8388608.f, 8388608.f));      // 2^23 + rn(65535 p)
+          pa[h][j] = __byte_perm(__float_as_uint(y.x), __float_as_uint(y.y), 0x5410);
         } else {
-          const uint2 w = lds8(v_tile + chunk_at<D>(key, g >> 1) + 8 * (g & 1));
-          v[r][0] = w.x; v[r][1] = w.y;
+          const __half2 packed = __floats2half2_rn(e.x, e.y);
+          pa[h][j] = *reinterpret_cast<const uint32_t*>(&packed);
         }
       }
+      sum[h] = fmaf(sum[h], shrink[h], part.x + part.y);
+    }
+
+    // ---- P.V: column n of output tile j is column n * D / 8 + j of V
+    if (!(ok = __all_sync(0xFFFFFFFFu, mbar_wait_timed(bar_v, n & 1u, abort_flag)))) break;
+    auto load_v = [&](uint32_t (&v)[D / 32], int key) {              // my D / 8 columns of a key
+      if constexpr (D == 128) {
+        const uint4 w = lds16(v_tile + chunk_at<D>(key, g));
+        v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
+      } else {
+        const uint2 w = lds8(v_tile + chunk_at<D>(key, g >> 1) + 8 * (g & 1));
+        v[0] = w.x; v[1] = w.y;
+      }
+    };
+    if constexpr (kEight) {
+      if (++held > kFlushTiles) { flush(1.f); held = 1; }
+      // 32 keys at a time: bytes 0-3 of a word of P are keys 2 t4, 2 t4 + 1, 8 + 2 t4 and 9 + 2 t4, of the second word 16 more
 #pragma unroll
-      for (int w = 0; w < D / 32; ++w) {
-        const uint32_t a = v[0][w] ^ 0x80808080u, b2 = v[1][w] ^ 0x80808080u, c = v[2][w] ^ 0x80808080u, d = v[3][w] ^ 0x80808080u;
-        const uint32_t ab01 = __byte_perm(a, b2, 0x5140), ab23 = __byte_perm(a, b2, 0x7362), cd01 = __byte_perm(c, d, 0x5140), cd23 = __byte_perm(c, d, 0x7362);
-        const uint32_t e = 0x64646464u;
-        mma16816(o[4 * w], pa[2 * kb][0], pa[2 * kb][1], pa[2 * kb + 1][0], pa[2 * kb + 1][1], sub1152(__byte_perm(ab01, e, 0x4140)), sub1152(__byte_perm(cd01, e, 0x4140)));
-        mma16816(o[4 * w + 1], pa[2 * kb][0], pa[2 * kb][1], pa[2 * kb + 1][0], pa[2 * kb + 1][1], sub1152(__byte_perm(ab01, e, 0x4342)), sub1152(__byte_perm(cd01, e, 0x4342)));
-        mma16816(o[4 * w + 2], pa[2 * kb][0], pa[2 * kb][1], pa[2 * kb + 1][0], pa[2 * kb + 1][1], sub1152(__byte_perm(ab23, e, 0x4140)), sub1152(__byte_perm(cd23, e, 0x4140)));
-        mma16816(o[4 * w + 3], pa[2 * kb][0], pa[2 * kb][1], pa[2 * kb + 1][0], pa[2 * kb + 1][1], sub1152(__byte_perm(ab23, e, 0x4342)), sub1152(__byte_perm(cd23, e, 0x4342)));
+      for (int kb = 0; kb < 4; ++kb) {
+        uint32_t a[4];                               // upper bytes, lower bytes of the first and of the second half of the keys
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          a[2 * y] = __byte_perm(pa[0][4 * kb + 2 * y], pa[0][4 * kb + 2 * y + 1], 0x7531);
+          a[2 * y + 1] = __byte_perm(pa[0][4 * kb + 2 * y], pa[0][4 * kb + 2 * y + 1], 0x6420);
+        }
+        uint32_t v[8][D / 32];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) load_v(v[r], 32 * kb + 2 * t4 + (r & 1) + 8 * (r >> 1));
+#pragma unroll
+        for (int w = 0; w < D / 32; ++w) {
+          uint32_t bytes[2][4];                      // bytes[y][i]: column 4 w + i of the four keys of half y
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const uint32_t t0 = __byte_perm(v[4 * y][w], v[4 * y + 1][w], 0x5140), t1 = __byte_perm(v[4 * y + 2][w], v[4 * y + 3][w], 0x5140);
+            const uint32_t t2 = __byte_perm(v[4 * y][w], v[4 * y + 1][w], 0x7362), t3 = __byte_perm(v[4 * y + 2][w], v[4 * y + 3][w], 0x7362);
+            bytes[y][0] = __byte_perm(t0, t1, 0x5410); bytes[y][1] = __byte_perm(t0, t1, 0x7632);
+            bytes[y][2] = __byte_perm(t2, t3, 0x5410); bytes[y][3] = __byte_perm(t2, t3, 0x7632);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mma16832_u(whole[4 * w + i], a[0], a[1], a[2], a[3], bytes[0][i], bytes[1][i]);
+        }
+      }
+    } else {
+      // sixteen keys at a time
+#pragma unroll
+      for (int kb = 0; kb < 8; ++kb) {
+        uint32_t v[4][D / 32];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) load_v(v[r], 16 * kb + 2 * t4 + (r & 1) + 8 * (r >> 1));
+#pragma unroll
+        for (int w = 0; w < D / 32; ++w) {
+          const uint32_t a = v[0][w] ^ 0x80808080u, b2 = v[1][w] ^ 0x80808080u, c = v[2][w] ^ 0x80808080u, d = v[3][w] ^ 0x80808080u, e = 0x64646464u;
+          const uint32_t ab[2] = {__byte_perm(a, b2, 0x5140), __byte_perm(a, b2, 0x7362)}, cd[2] = {__byte_perm(c, d, 0x5140), __byte_perm(c, d, 0x7362)};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t pick = (i & 1) ? 0x4342 : 0x4140;
+            float acc[4] = {o[0][4 * w + i][0], o[0][4 * w + i][1], o[kHalves - 1][4 * w + i][0], o[kHalves - 1][4 * w + i][1]};
+            mma16816(acc, pa[0][2 * kb], pa[kHalves - 1][2 * kb], pa[0][2 * kb + 1], pa[kHalves - 1][2 * kb + 1], sub1152(__byte_perm(ab[i >> 1], e, pick)),
+                     sub1152(__byte_perm(cd[i >> 1], e, pick)));
+            o[0][4 * w + i][0] = acc[0]; o[0][4 * w + i][1] = acc[1];
+            o[kHalves - 1][4 * w + i][0] = acc[2]; o[kHalves - 1][4 * w + i][1] = acc[3];
+          }
+        }
       }
     }
     __syncwarp();
@@ -240,17 +329,18 @@ rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
   if (bad_page) report(p.status, p.host_word, FMHA_I8_DEV_BAD_INDEX, 1u, b);
 
   // ---- the warp's partial rows go over its own tiles, which it has done with
+  if constexpr (kEight) flush(1.f);
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+  for (int h = 0; h < kHalves; ++h) {
     sum[h] += __shfl_xor_sync(0xFFFFFFFFu, sum[h], 1);
     sum[h] += __shfl_xor_sync(0xFFFFFFFFu, sum[h], 2);
     if (t4 == 0) sm.stat[warp][g + 8 * h] = make_float2(ref[h], sum[h]);
     float* dst = reinterpret_cast<float*>(sm.ring + warp * 2 * C::kTileBytes) + (g + 8 * h) * D + t4 * (D / 4);
 #pragma unroll
-    for (int x = 0; x < 2; ++x)                      // columns n = 2 t4 + x: D / 8 neighbours
+    for (int y = 0; y < 2; ++y)                      // columns n = 2 t4 + y: D / 8 neighbours
 #pragma unroll
       for (int j = 0; j < kOut; j += 4)
-        *reinterpret_cast<float4*>(dst + x * (D / 8) + j) = make_float4(o[j][2 * h + x], o[j + 1][2 * h + x], o[j + 2][2 * h + x], o[j + 3][2 * h + x]);
+        *reinterpret_cast<float4*>(dst + y * (D / 8) + j) = make_float4(o[h][j][y], o[h][j + 1][y], o[h][j + 2][y], o[h][j + 3][y]);
   }
   cluster_arrive();
   cluster_wait();
@@ -259,16 +349,16 @@ rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
   const int parts = ctas * W;
   for (int i = threadIdx.x; i < kRows; i += W * 32) {
     float m = -INFINITY, l = 0.f;
-    for (int x = 0; x < parts; ++x) m = fmaxf(m, ld_cluster_v2(map_to_rank(smem_u32(&sm.stat[x % W][i]), x / W)).x);
+    for (int y = 0; y < parts; ++y) m = fmaxf(m, ld_cluster_v2(map_to_rank(smem_u32(&sm.stat[y % W][i]), y / W)).x);
     const float base = m == -INFINITY ? 0.f : m;
-    for (int x = 0; x < parts; ++x) {
-      const float2 st = ld_cluster_v2(map_to_rank(smem_u32(&sm.stat[x % W][i]), x / W));
-      const float e = ex2(st.x - base);
+    for (int y = 0; y < parts; ++y) {
+      const float2 st = ld_cluster_v2(map_to_rank(smem_u32(&sm.stat[y % W][i]), y / W));
+      const float e = ex2((st.x - base) * p.c2);
       l = fmaf(e, st.y, l);
-      sm.weight[x][i] = e;
+      sm.weight[y][i] = e;
     }
-    const float inv = l > 0.f ? p.out_scale / l : 0.f;
-    for (int x = 0; x < parts; ++x) sm.weight[x][i] *= inv;
+    const float inv = l > 0.f ? p.out_scale / (kEight ? l * kLevels : l) : 0.f;
+    for (int y = 0; y < parts; ++y) sm.weight[y][i] *= inv;
   }
   __syncthreads();
   constexpr int kQuads = D / 4;
@@ -276,10 +366,10 @@ rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
     const int r = i / kQuads, c = i % kQuads, row = row0 + r;
     if (row >= n_rows) break;
     float a[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int x = 0; x < parts; ++x) {
-      const float e = sm.weight[x][r];
+    for (int y = 0; y < parts; ++y) {
+      const float e = sm.weight[y][r];
       if (e == 0.f) continue;                        // a warp without keys for this row
-      const float4 v = ld_cluster_v4(map_to_rank(smem_u32(sm.ring + (x % W) * 2 * C::kTileBytes) + static_cast<uint32_t>((r * D + 4 * c) * 4), x / W));
+      const float4 v = ld_cluster_v4(map_to_rank(smem_u32(sm.ring + (y % W) * 2 * C::kTileBytes) + static_cast<uint32_t>((r * D + 4 * c) * 4), y / W));
       a[0] = fmaf(e, v.x, a[0]); a[1] = fmaf(e, v.y, a[1]); a[2] = fmaf(e, v.z, a[2]); a[3] = fmaf(e, v.w, a[3]);
     }
     const int token = row / p.G;

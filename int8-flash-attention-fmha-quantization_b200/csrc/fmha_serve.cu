@@ -63,17 +63,21 @@ int launch(void (*fn)(Params...), unsigned grid, unsigned block, size_t smem, cu
 
 template <int D> using RowsCfg = rows::Cfg<D>;
 
-template <int D> int set_up_rows(int* clusters16) {
+template <int D, int kRows> int set_up_rows() {
   constexpr int W = RowsCfg<D>::kWarps, Wide = RowsCfg<D>::kWarpsWide;
   auto set = [](const void* fn, size_t bytes) {
     return cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) == cudaSuccess &&
            cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess;
   };
-  if (!set(reinterpret_cast<const void*>(&rows::rows_kernel<D, W>), sizeof(rows::Smem<D, W>)) ||
-      !set(reinterpret_cast<const void*>(&rows::rows_kernel<D, Wide>), sizeof(rows::Smem<D, Wide>))) {
-    cudaGetLastError();
-    return FMHA_I8_ERR_LAUNCH;
-  }
+  if (set(reinterpret_cast<const void*>(&rows::rows_kernel<D, W, kRows>), sizeof(rows::Smem<D, W, kRows>)) &&
+      set(reinterpret_cast<const void*>(&rows::rows_kernel<D, Wide, kRows>), sizeof(rows::Smem<D, Wide, kRows>)))
+    return FMHA_I8_OK;
+  cudaGetLastError();
+  return FMHA_I8_ERR_LAUNCH;
+}
+// Clusters of 16 CTAs of the wide kernel that are resident at once.
+template <int D> int count_clusters() {
+  constexpr int Wide = RowsCfg<D>::kWarpsWide;
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -81,12 +85,13 @@ template <int D> int set_up_rows(int* clusters16) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.gridDim = dim3(16);
   cfg.blockDim = dim3(Wide * 32);
-  cfg.dynamicSmemBytes = sizeof(rows::Smem<D, Wide>);
+  cfg.dynamicSmemBytes = sizeof(rows::Smem<D, Wide, 16>);
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (cudaOccupancyMaxActiveClusters(clusters16, rows::rows_kernel<D, Wide>, &cfg) != cudaSuccess) *clusters16 = 0;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, rows::rows_kernel<D, Wide, 16>, &cfg) != cudaSuccess) n = 0;
   cudaGetLastError();
-  return FMHA_I8_OK;
+  return n;
 }
 
 template <int D> int set_up_chunk() {
@@ -111,8 +116,10 @@ int set_up(const Device& dev) {
   std::lock_guard<std::mutex> lock(g_once_mutex);
   if (once.done.load(std::memory_order_relaxed)) return FMHA_I8_OK;
   int st;
-  if ((st = set_up_rows<64>(&once.clusters16_d64)) != FMHA_I8_OK) return st;
-  if ((st = set_up_rows<128>(&once.clusters16_d128)) != FMHA_I8_OK) return st;
+  if ((st = set_up_rows<64, 8>()) != FMHA_I8_OK || (st = set_up_rows<64, 16>()) != FMHA_I8_OK) return st;
+  if ((st = set_up_rows<128, 8>()) != FMHA_I8_OK || (st = set_up_rows<128, 16>()) != FMHA_I8_OK) return st;
+  once.clusters16_d64 = count_clusters<64>();
+  once.clusters16_d128 = count_clusters<128>();
   if ((st = set_up_chunk<64>()) != FMHA_I8_OK || (st = set_up_chunk<128>()) != FMHA_I8_OK) return st;
   once.done.store(true, std::memory_order_release);
   return FMHA_I8_OK;
@@ -182,10 +189,10 @@ int fill_call(Call* c, const float amax[5], const int desc6[6], const void* q, c
   return FMHA_I8_OK;
 }
 
-template <int D> int launch_rows(cudaStream_t stream, const Device& dev, Call& c, const CUtensorMap& mk, const CUtensorMap& mv) {
+template <int D, int kRows> int launch_rows(cudaStream_t stream, const Device& dev, Call& c, const CUtensorMap& mk, const CUtensorMap& mv) {
   grouped::Params& p = c.p;
   constexpr int W = RowsCfg<D>::kWarps, Wide = RowsCfg<D>::kWarpsWide;
-  p.row_groups = static_cast<int>((static_cast<long long>(p.max_q) * p.G + rows::kRows - 1) / rows::kRows);
+  p.row_groups = static_cast<int>((static_cast<long long>(p.max_q) * p.G + kRows - 1) / kRows);
   const long long units = static_cast<long long>(p.B) * p.Hkv * p.row_groups;
   const long long n_tiles = (c.max_k + grouped::kTile - 1) / grouped::kTile;
   if (units > kMostRows / rows::kMaxCluster) return FMHA_I8_ERR_TOO_LARGE;
@@ -194,13 +201,13 @@ template <int D> int launch_rows(cudaStream_t stream, const Device& dev, Call& c
   while (ctas < 8 && ((units * ctas < 2 * resident && n_tiles >= 4 * ctas * W) || (units * ctas * 2 <= resident && n_tiles >= 2 * ctas * W))) ctas *= 2;
   const int clusters16 = D == 128 ? g_once[dev.index].clusters16_d128 : g_once[dev.index].clusters16_d64;
   if (ctas == 8 && units <= clusters16 && n_tiles >= 32 * Wide)
-    return launch(rows::rows_kernel<D, Wide>, static_cast<unsigned>(units * 16), Wide * 32, sizeof(rows::Smem<D, Wide>), stream, 16u, mk, mv, p);
-  return launch(rows::rows_kernel<D, W>, static_cast<unsigned>(units * ctas), W * 32, sizeof(rows::Smem<D, W>), stream, static_cast<unsigned>(ctas), mk, mv, p);
+    return launch(rows::rows_kernel<D, Wide, kRows>, static_cast<unsigned>(units * 16), Wide * 32, sizeof(rows::Smem<D, Wide, kRows>), stream, 16u, mk, mv, p);
+  return launch(rows::rows_kernel<D, W, kRows>, static_cast<unsigned>(units * ctas), W * 32, sizeof(rows::Smem<D, W, kRows>), stream, static_cast<unsigned>(ctas), mk, mv, p);
 }
 
 // Up to 128 heads share a key head, and a tile of the chunk kernel holds at least one token.
 constexpr int kMostGroup = 128;
-bool few_rows(const grouped::Params& p) { return p.G > kMostGroup || static_cast<long long>(p.max_q) * p.G <= rows::kRows; }
+bool few_rows(const grouped::Params& p) { return p.G > kMostGroup || static_cast<long long>(p.max_q) * p.G <= 16; }
 
 template <int D> int launch_chunk(cudaStream_t stream, const Device& dev, Call& c, const CUtensorMap& mk, const CUtensorMap& mv) {
   grouped::Params& p = c.p;
@@ -232,7 +239,10 @@ int run_attention(void* stream, Call& c) {
   if ((st = key_map(&mk, c.k, c.lk, c.D)) != FMHA_I8_OK) return st;
   if ((st = key_map(&mv, c.v, c.lv, c.D)) != FMHA_I8_OK) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (few_rows(c.p)) return c.D == 128 ? launch_rows<128>(s, dev, c, mk, mv) : launch_rows<64>(s, dev, c, mk, mv);
+  if (few_rows(c.p)) {
+    if (static_cast<long long>(c.p.max_q) * c.p.G <= 8) return c.D == 128 ? launch_rows<128, 8>(s, dev, c, mk, mv) : launch_rows<64, 8>(s, dev, c, mk, mv);
+    return c.D == 128 ? launch_rows<128, 16>(s, dev, c, mk, mv) : launch_rows<64, 16>(s, dev, c, mk, mv);
+  }
   return c.D == 128 ? launch_chunk<128>(s, dev, c, mk, mv) : launch_chunk<64>(s, dev, c, mk, mv);
 }
 

@@ -22,12 +22,13 @@ def starts(lengths, device="cuda"):
 
 
 def attention64(q, k, v, amax, causal):
-    """One sequence: q [n, H, D], k, v [m, Hkv, D] int8 -> (o, spread) float64 [n, H, D]: the output in real units and the tolerance's
-    scale, sum_j p_j |v_j| (see tolerance())."""
+    """One sequence: q [n, H, D], k, v [m, Hkv, D] int8 -> (o, scales): float64 [n, H, D], the output in real units, and two of that shape for
+    tolerance(): sum_j p_j |v_j| with the p of a row adding up to 1, and sum_j |v_j| / sum_j p_j over the keys that the row sees, the largest p being 1."""
     n, H, D = q.shape
     m, Hkv = k.shape[0], k.shape[1]
     if n == 0 or m == 0:
-        return (torch.zeros((n, H, D), dtype=torch.float64, device=q.device),) * 2
+        none = torch.zeros((n, H, D), dtype=torch.float64, device=q.device)
+        return none, (none, none)
     scale = float(torch.tensor(amax[0])) * float(torch.tensor(amax[1])) / 127.0 ** 2 / math.sqrt(D)
     kk, vv = (x.double().repeat_interleave(H // Hkv, 1).transpose(0, 1) for x in (k, v))
     s = q.double().transpose(0, 1) @ kk.transpose(1, 2) * scale
@@ -40,30 +41,33 @@ def attention64(q, k, v, amax, causal):
     l = p.sum(-1, keepdim=True)
     p = torch.where(l > 0, p / torch.where(l > 0, l, 1.0), 0.0)
     real = float(torch.tensor(amax[2])) / 127.0
-    return (p @ vv).transpose(0, 1) * real, (p @ vv.abs()).transpose(0, 1) * real
+    each = torch.where(l > 0, (seen.double() @ vv.abs()) / torch.where(l > 0, l, 1.0), 0.0)
+    return (p @ vv).transpose(0, 1) * real, ((p @ vv.abs()).transpose(0, 1) * real, each.transpose(0, 1) * real)
 
 
-def tolerance(o, spread, keys, o_type, amax, o_amax):
-    """Elementwise bound of |result - o|, o in real units.
-      P        fp16: half a step, 2^-11 relative, of every p: 2^-11 sum p |v|; below 2^-14 half a step is 2^-25, absolute, where the row's largest p is 1 or
-               more, so that the sum of p is too: keys * 2^-25 * v_amax.
-      exp2     2^-22; its argument (|a| <= 24 where p matters to fp16) is off by half a step of the factor (22 bits: 2^-23 relative), of the factor's own
-               formula in fp32 (2^-24) and of its rounding (2^-24): 24 * 2^-22 * ln 2 < 2^-17.9; with the rest 2^-17.8 together.
+def tolerance(o, scales, keys, o_type, amax, o_amax, rows):
+    """Elementwise bound of |result - o|, o in real units.  `rows`: query rows per key head that the call allows (max_seq_q * heads of a group).
+      P        fp16: half a step, 2^-11 relative, of every p; below 2^-14 half a step is 2^-25 of the row's largest p, which is 1 or more.  Up to eight rows: whole
+               numbers of 16 bits, half a step, 2^-17 of the largest p, for every key.
+      exp2     2^-22; its argument (|a| <= 24 where p matters) is off by half a step of the factor and of its rounding (2^-24 relative each) and, up to
+               eight rows, of a difference: 24 * 3 * 2^-24 * ln 2 < 2^-18.3; with the rest 2^-18 together.
       sums     keys additions in fp32, half a step (2^-24) each, of sums at most sum p |v|.
       output   half a step of its type relative to the result (int8: half a code)."""
     out = torch.full_like(o, 0.5 * o_amax / 127.0) if o_type == "int8" else o.abs() * (torch.finfo(TYPES[o_type]).eps / 2)
     tiny = 0.0 if o_type != "fp16" else 2.0 ** -25            # half a step below fp16's smallest normal number
-    return out * 1.001 + spread * (2.0 ** -11 + 2.0 ** -17.8 + keys * 2.0 ** -24) + keys * 2.0 ** -25 * amax[2] + tiny
+    spread, each = scales
+    of_p = each * 2.0 ** -17 if rows <= 8 else spread * 2.0 ** -11 + each * 2.0 ** -25
+    return out * 1.001 + of_p + spread * (2.0 ** -18 + keys * 2.0 ** -24) + tiny + 1e-12
 
 
 def real_units(o, o_type, o_amax):
     return o.double() * (o_amax / 127.0) if o_type == "int8" else o.double()
 
 
-def check(got, want, spread, keys, o_type, amax, o_amax, what=""):
+def check(got, want, scales, keys, o_type, amax, o_amax, rows, what=""):
     want_c = want.clamp(-o_amax, o_amax) if o_type == "int8" else want
     err = (real_units(got, o_type, o_amax) - want_c).abs()
-    tol = tolerance(want_c, spread, keys, o_type, amax, o_amax)
+    tol = tolerance(want_c, scales, keys, o_type, amax, o_amax, rows)
     over = err > tol
     assert not bool(over.any()), f"{what}: {int(over.sum())} of {over.numel()} off, worst {float((err / tol).max()):.3g} times the tolerance"
 

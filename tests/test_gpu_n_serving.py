@@ -171,7 +171,7 @@ def run_packed(pkg, torch, lens_q, lens_k, H, Hkv, D, causal, out, seed, tail=3,
     at_q = at_k = 0
     for n, m in zip(lens_q, lens_k):
         want, spread = attention64(q[at_q:at_q + n], k[at_k:at_k + m], v[at_k:at_k + m], AMAX, causal)
-        check(o[at_q:at_q + n], want, spread, m, out, AMAX, O_AMAX, f"{n} tokens on {m} keys")
+        check(o[at_q:at_q + n], want, spread, m, out, AMAX, O_AMAX, desc.max_seq_q * H // Hkv, f"{n} tokens on {m} keys")
         at_q += n
         at_k += m
     assert bool((o[at_q:] == FILL[out]).all()), "tokens behind the last sequence were touched"
@@ -226,7 +226,7 @@ def test_packed_rows_that_are_far_from_even(pkg, torch):
         cu = starts([150])
         pkg.FMHAInferI8Packed(None, pkg.FMHAParamI8(*amax, 1.0, 1.0), pkg.AttnDataDescriptorGrouped(1, 150, 150, 4, 2, 64), q, k, v, cu, cu, o)
         want, spread = attention64(q, k, v, amax, True)
-        check(o, want, spread, 150, "bf16", amax, 1.0, str(a))
+        check(o, want, spread, 150, "bf16", amax, 1.0, 300, str(a))
 
 
 def test_packed_identical_scores_and_growing_maxima(pkg, torch):
@@ -242,12 +242,12 @@ def test_packed_identical_scores_and_growing_maxima(pkg, torch):
         o = torch.empty((1, 1, D), dtype=torch.float16, device="cuda")
         pkg.FMHAInferI8Packed(None, param(pkg), pkg.AttnDataDescriptorGrouped(1, 1, n, 1, 1, D), q, k, v, starts([1]), starts([n]), o)
         want, spread = attention64(q, k, v, AMAX, True)
-        check(o, want, spread, n, "fp16", AMAX, 1.0, str(step))
+        check(o, want, spread, n, "fp16", AMAX, 1.0, 1, str(step))
         rows = q.expand(400, 1, D).contiguous()
         o = torch.empty((400, 1, D), dtype=torch.float16, device="cuda")
         pkg.FMHAInferI8Packed(None, param(pkg), pkg.AttnDataDescriptorGrouped(1, 400, n, 1, 1, D), rows, k, v, starts([400]), starts([n]), o)
         want, spread = attention64(rows, k, v, AMAX, True)
-        check(o, want, spread, n, "fp16", AMAX, 1.0, str(step))
+        check(o, want, spread, n, "fp16", AMAX, 1.0, 400, str(step))
 
 
 def test_packed_offsets_outside_the_tensors_are_cut_and_reported(pkg, torch):
@@ -304,7 +304,7 @@ def run_paged(pkg, torch, lens_q, lens_k, H, Hkv, D, page, out, seed, causal=Tru
     at = 0
     for b, (n, m) in enumerate(zip(lens_q, lens_k)):
         want, spread = attention64(q[at:at + n], keys_of(kc, table, b, m), keys_of(vc, table, b, m), AMAX, causal)
-        check(o[at:at + n], want, spread, m, out, AMAX, O_AMAX, f"sequence {b}: {n} tokens on {m} keys")
+        check(o[at:at + n], want, spread, m, out, AMAX, O_AMAX, desc.max_seq_q * H // Hkv, f"sequence {b}: {n} tokens on {m} keys")
         at += n
     assert bool((o[at:] == FILL[out]).all())
 
@@ -352,12 +352,12 @@ def test_paged_pages_and_lengths_outside_are_reported(pkg, torch):
         st, words = pkg.device_status()
         assert st == pkg.ERR_DEVICE and words[0] == 13 and words[2] == 1, (bad, words)
         want, spread = attention64(q[1:], keys_of(kc, table, 1, 40), keys_of(vc, table, 1, 40), AMAX, True)
-        check(o[1:], want, spread, 40, "bf16", AMAX, O_AMAX)
+        check(o[1:], want, spread, 40, "bf16", AMAX, O_AMAX, 1)
     for length in (table.shape[1] * 16 + 1, -1):
         pkg.FMHAInferI8Paged(None, param(pkg), desc, q, kc, vc, table.clamp(min=0), torch.tensor([length, 40], dtype=torch.int32, device="cuda"), starts([1, 1]), o)
         st, words = pkg.device_status()
         assert st == pkg.ERR_DEVICE and words[0] == 13 and words[2] == 0, words
-        check(o[1:], want, spread, 40, "bf16", AMAX, O_AMAX)
+        check(o[1:], want, spread, 40, "bf16", AMAX, O_AMAX, 1)
 
 
 def test_paged_offsets_beyond_32_bits(pkg, torch):
@@ -378,7 +378,7 @@ def test_paged_offsets_beyond_32_bits(pkg, torch):
         pkg.FMHAInferI8Paged(None, param(pkg), pkg.AttnDataDescriptorGrouped(1, n_q, n, Hkv * g, Hkv, D), q, kc, vc, table,
                              torch.tensor([n], dtype=torch.int32, device="cuda"), starts([n_q]), o)
         want, spread = attention64(q, k, v, AMAX, True)
-        check(o, want, spread, n, "bf16", AMAX, O_AMAX)
+        check(o, want, spread, n, "bf16", AMAX, O_AMAX, n_q * g)
 
 
 # ------------------------------------------------------------------------------------------------ together, as they are used
@@ -397,24 +397,26 @@ def test_prefill_then_chunks_then_single_tokens_agree(pkg, torch):
     pkg.FMHAInferI8Packed(None, param(pkg), pkg.AttnDataDescriptorGrouped(1, T, T, H, Hkv, D), q8, k8, v8, cu, cu, whole)
     want_q, want_k = (quantise64(rotate64(x.double(), pos, freq, 1.0, False), a) for x, a in ((qf, AMAX[0]), (kf, AMAX[1])))
     want, spread = attention64(want_q, want_k, quantise64(vf.double(), AMAX[2]), AMAX, True)
-    check(whole, want, spread, T, "bf16", AMAX, 1.0)
+    check(whole, want, spread, T, "bf16", AMAX, 1.0, T * H // Hkv)
 
     pages = -(-T // page)
     kc, vc = (torch.zeros((pages + 1, Hkv, page, D), dtype=torch.int8, device="cuda") for _ in range(2))
     page_table = torch.randperm(pages + 1, device="cuda")[:pages].to(torch.int32)[None]
     out = torch.empty_like(whole)
-    at = 0
+    at, rows_of = 0, []
     for n in (129, 70, 33, 3) + (1,) * 65:
         rows = slice(at, at + n)
         where = torch.arange(at, at + n, device="cuda")
         slots = page_table[0, where // page].long() * page + where % page
         qn = torch.empty((n, H, D), dtype=torch.int8, device="cuda")
         pkg.rope_quantize_append(None, param(pkg), qf[rows], kf[rows], vf[rows], pos[rows], table, qn, kc, vc, slots=slots)
+        rows_of.append((rows, n * H // Hkv))
         at += n
         pkg.FMHAInferI8Paged(None, param(pkg), pkg.AttnDataDescriptorGrouped(1, n, at, H, Hkv, D), qn, kc, vc, page_table,
                              torch.tensor([at], dtype=torch.int32, device="cuda"), starts([n]), out[rows])
     assert at == T
-    check(out, want, spread, T, "bf16", AMAX, 1.0)
+    for rows, n in rows_of:
+        check(out[rows], want[rows], tuple(x[rows] for x in spread), T, "bf16", AMAX, 1.0, n)
 
 
 def test_a_captured_step_follows_lengths_and_pages(pkg, torch):
@@ -456,7 +458,7 @@ def test_a_captured_step_follows_lengths_and_pages(pkg, torch):
         torch.cuda.synchronize()
         for b, n in enumerate(new):
             want, spread = attention64(q8[b:b + 1], keys_of(kc, table, b, n), keys_of(vc, table, b, n), AMAX, True)
-            check(o[b:b + 1], want, spread, n, "bf16", AMAX, O_AMAX, f"replay {i}")
+            check(o[b:b + 1], want, spread, n, "bf16", AMAX, O_AMAX, H // Hkv, f"replay {i}")
             assert torch.equal(keys_of(vc, table, b, n)[-1], quantise64(qkv[b, H + Hkv:].double(), AMAX[2]))
 
 
