@@ -27,7 +27,7 @@ struct Params {
   long long q_stride, k_stride, v_stride;      // elements from one token to the next
   long long page_stride, num_slots;
   int page_shift;
-  int tokens, H, Hkv, rot, interleaved;
+  int tokens, H, Hkv, rot;
   int rounds;                          // a warp goes over rounds * (heads that it takes at once) heads of a token
   int parts;                           // warps per token
   float amax[3], scale[3];             // ranges of q, k, v, and 127 / range
@@ -35,113 +35,143 @@ struct Params {
   unsigned* host_word;
 };
 
-// Sixteen elements of one head: eight and eight.
-template <typename T> struct Load;
-template <> struct Load<float> {
-  static __device__ __forceinline__ void eight(const float* at, float (&x)[8]) {
-    const float4 a = reinterpret_cast<const float4*>(at)[0], b = reinterpret_cast<const float4*>(at)[1];
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+// Eight neighbouring elements as they are in memory, and as four pairs of floats.
+template <typename T> struct Eight { uint4 w; };
+template <> struct Eight<float> { float4 w[2]; };
+template <typename T> __device__ __forceinline__ void load8(const T* at, Eight<T>& e) {
+  if constexpr (sizeof(T) == 4) {
+    e.w[0] = reinterpret_cast<const float4*>(at)[0];
+    e.w[1] = reinterpret_cast<const float4*>(at)[1];
+  } else {
+    e.w = *reinterpret_cast<const uint4*>(at);
   }
-};
-template <> struct Load<__nv_bfloat16> {
-  static __device__ __forceinline__ void eight(const __nv_bfloat16* at, float (&x)[8]) {
-    const uint4 w = *reinterpret_cast<const uint4*>(at);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(u[i] << 16); x[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u); }
+}
+__device__ __forceinline__ float2 pair_of(uint32_t u, __nv_bfloat16) { return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u)); }
+__device__ __forceinline__ float2 pair_of(uint32_t u, __half) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
+template <typename T> __device__ __forceinline__ void floats(const Eight<T>& e, float2 (&x)[4]) {
+  if constexpr (sizeof(T) == 4) {
+    x[0] = make_float2(e.w[0].x, e.w[0].y); x[1] = make_float2(e.w[0].z, e.w[0].w);
+    x[2] = make_float2(e.w[1].x, e.w[1].y); x[3] = make_float2(e.w[1].z, e.w[1].w);
+  } else {
+    x[0] = pair_of(e.w.x, T()); x[1] = pair_of(e.w.y, T()); x[2] = pair_of(e.w.z, T()); x[3] = pair_of(e.w.w, T());
   }
-};
-template <> struct Load<__half> {
-  static __device__ __forceinline__ void eight(const __half* at, float (&x)[8]) {
-    const uint4 w = *reinterpret_cast<const uint4*>(at);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
-      x[2 * i] = f.x; x[2 * i + 1] = f.y;
-    }
-  }
-};
+}
 
 // The code of y in 64 bits: the definition.
 __device__ __forceinline__ float code_exact(double y, double scale) {
   const double z = floor(__dadd_rn(__dmul_rn(y, scale), 0.5));
   return z == z ? static_cast<float>(fmin(fmax(z, -127.0), 127.0)) : 0.f;
 }
-// Codes of eight values y (as floats plus kMagic), whose errors are at most `error` in codes.  False if one of them may be another.
-__device__ __forceinline__ bool codes_fast(const float (&y)[8], float scale, float error, float (&code)[8]) {
-  float least = 1.f, most = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    // between -127 and -126, and from 127 on, the code is the same; the clamped values lie in the middle of those
-    const float z = fminf(fmaxf(fmaf(y[i], scale, 0.5f), -126.5f), 127.5f);
-    code[i] = __fadd_rd(z, kMagic);
-    const float part = z - (code[i] - kMagic);         // exact
-    least = fminf(least, part);
-    most = fmaxf(most, part);
-  }
-  return least > error && most < 1.f - error;
-}
-__device__ __forceinline__ uint2 pack8(const float (&c)[8]) {
-  auto word = [&](int i) {
-    return __byte_perm(__byte_perm(__float_as_uint(c[i]), __float_as_uint(c[i + 1]), 0x0040),
-                       __byte_perm(__float_as_uint(c[i + 2]), __float_as_uint(c[i + 3]), 0x0040), 0x5410);
+__device__ __forceinline__ uint2 pack8(const float2 (&c)[4]) {
+  auto word = [&](const float2& a, const float2& b) {
+    return __byte_perm(__byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0040), __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040), 0x5410);
   };
-  return make_uint2(word(0), word(4));
+  return make_uint2(word(c[0], c[1]), word(c[2], c[3]));
+}
+__device__ __forceinline__ float max_abs(float m, const float2 (&x)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = max3_abs_nan(m, x[i].x, x[i].y);
+  return m;
 }
 
-// Sixteen elements, a and b: with kRotate pairs -- (a[i], b[i]), or interleaved neighbours in a and then in b -- are turned by cs; otherwise
-// they are quantised as they are.  `low`: second plane of the table for these pairs.
-template <bool kRotate>
-__device__ __forceinline__ void quantise16(const float (&a)[8], const float (&b)[8], const float2 (&cs)[8], float most_cs, const float* low, bool interleaved, float amax, float scale,
-                                           uint2& first, uint2& second) {
-  float ya[8], yb[8], most = 0.f;
+// What a thread knows of the rotations of its eight pairs.
+struct Turn {
+  float2 c[4], s[4];                   // cosines and sines of pairs 2 i and 2 i + 1
+  float most;                          // the largest of them
+  const float* low;                    // second plane of the table
+};
+__device__ __forceinline__ float at(const float2 (&x)[4], int i) { return (i & 1) ? x[i >> 1].y : x[i >> 1].x; }
+
+// Sixteen elements, a and b.  With kTurn they are eight pairs -- (a[i], b[i]), or interleaved neighbours in a and then in b -- and are turned.
+template <bool kTurn, bool kInterleaved>
+__device__ __forceinline__ void quantise16(float2 (&a)[4], float2 (&b)[4], const Turn& turn, float amax, float scale, uint2& first, uint2& second) {
+  const float most = max_abs(max_abs(0.f, a), b);
+  float2 y[2][4];
+  if constexpr (kTurn && !kInterleaved) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) most = max3_abs_nan(most, a[i], b[i]);
-  if constexpr (kRotate) {
+    for (int i = 0; i < 4; ++i) {
+      const float2 t = __fmul2_rn(b[i], turn.s[i]);
+      y[0][i] = __ffma2_rn(a[i], turn.c[i], make_float2(-t.x, -t.y));
+      y[1][i] = __ffma2_rn(b[i], turn.c[i], __fmul2_rn(a[i], turn.s[i]));
+    }
+  } else if constexpr (kTurn) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float x1 = !interleaved ? a[i] : i < 4 ? a[2 * i] : b[2 * i - 8], x2 = !interleaved ? b[i] : i < 4 ? a[2 * i + 1] : b[2 * i - 7];
-      const float y1 = fmaf(x1, cs[i].x, -__fmul_rn(x2, cs[i].y)), y2 = fmaf(x2, cs[i].x, __fmul_rn(x1, cs[i].y));
-      if (!interleaved) { ya[i] = y1; yb[i] = y2; }
-      else if (i < 4) { ya[2 * i] = y1; ya[2 * i + 1] = y2; }
-      else { yb[2 * i - 8] = y1; yb[2 * i - 7] = y2; }
+      const float2 v = i < 4 ? a[i] : b[i - 4];
+      const float c = at(turn.c, i), s = at(turn.s, i);
+      y[i >> 2][i & 3] = make_float2(fmaf(v.x, c, -__fmul_rn(v.y, s)), fmaf(v.y, c, __fmul_rn(v.x, s)));
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) { ya[i] = a[i]; yb[i] = b[i]; }
+    for (int i = 0; i < 4; ++i) { y[0][i] = a[i]; y[1][i] = b[i]; }
   }
-  // With m the largest |x| and c the largest |cos|, |sin| here, a product is at most m c.  y1: half a step (2^-24) of each of table, product, and sum
-  // of two: 2^-24 (2 + 1 + 2) m c; times the scale, itself half a step off (2^-24 of at most 2 m c); and half a step of the result, which counts only
-  // below 128 (2^-17).  Together 7 * 2^-24 m c scale + 2^-17 / 2 codes; taken: 2^-21 m c scale + 2^-17.
-  const float error = fmaf(most * most_cs * scale, 0x1p-21f, 0x1p-17f);
-  float ca[8], cb[8];
-  const bool sure_a = codes_fast(ya, scale, error, ca), sure_b = codes_fast(yb, scale, error, cb);
-  if (!(sure_a && sure_b)) {
-    const double scale64 = 127.0 / static_cast<double>(amax);
-    if constexpr (kRotate) {
+  // With m the largest |x| and c the largest |cos|, |sin| here, a product is at most m c.  Half a step (2^-24) of each of table, product, and sum
+  // of two: 2^-24 (2 + 1 + 2) m c; times the scale, itself half a step off (2^-24 of at most 2 m c); and half a step of the result, at most 2^-18 below
+  // 128.  Together 7 * 2^-24 m c scale + 2^-18 codes; taken: 2^-21 m c scale + 2^-17.
+  const float error = fmaf(most * (kTurn ? turn.most : 1.f) * scale, 0x1p-21f, 0x1p-17f);
+  // z and the whole number next to it, as kMagic + n: rounded to nearest, which is floor(z + 1/2) unless z lies half way between two.
+  const float2 scale2 = make_float2(scale, scale), magic = make_float2(kMagic, kMagic), less = make_float2(-kMagic, -kMagic);
+  float2 code[2][4];
+  float off = 0.f, largest = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const double c = static_cast<double>(cs[i].x) + static_cast<double>(low[2 * i]), s = static_cast<double>(cs[i].y) + static_cast<double>(low[2 * i + 1]);
-        const double x1 = !interleaved ? a[i] : i < 4 ? a[2 * i] : b[2 * i - 8], x2 = !interleaved ? b[i] : i < 4 ? a[2 * i + 1] : b[2 * i - 7];
-        const float y1 = kMagic + code_exact(__dadd_rn(__dmul_rn(x1, c), -__dmul_rn(x2, s)), scale64);
-        const float y2 = kMagic + code_exact(__dadd_rn(__dmul_rn(x2, c), __dmul_rn(x1, s)), scale64);
-        if (!interleaved) { ca[i] = y1; cb[i] = y2; }
-        else if (i < 4) { ca[2 * i] = y1; ca[2 * i + 1] = y2; }
-        else { cb[2 * i - 8] = y1; cb[2 * i - 7] = y2; }
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 z = __fmul2_rn(y[h][i], scale2);
+      code[h][i] = __fadd2_rn(z, magic);
+      const float2 n = __fadd2_rn(code[h][i], less), d = __fadd2_rn(z, make_float2(-n.x, -n.y));
+      off = max3_abs_nan(off, d.x, d.y);
+      largest = max3_abs_nan(largest, z.x, z.y);
+    }
+  if (!(largest < 127.25f)) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        code[h][i].x = fminf(fmaxf(code[h][i].x, kMagic - 127.f), kMagic + 127.f);
+        code[h][i].y = fminf(fmaxf(code[h][i].y, kMagic - 127.f), kMagic + 127.f);
       }
-    } else {
+  }
+  // (beyond 2^22 a float next to kMagic has no room for n; d is then as large as z or not a number)
+  if (!(off < 0.5f - error)) {
+    const double scale64 = 127.0 / static_cast<double>(amax);
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) {
+      double x1, x2, c = 1.0, s = 0.0;
+      if (kTurn && kInterleaved) {
+        const float2 v = i < 4 ? (i < 2 ? (i == 0 ? a[0] : a[1]) : (i == 2 ? a[2] : a[3])) : (i < 6 ? (i == 4 ? b[0] : b[1]) : (i == 6 ? b[2] : b[3]));
+        x1 = v.x; x2 = v.y;
+      } else {
+        const float2 va = i < 4 ? (i < 2 ? a[0] : a[1]) : (i < 6 ? a[2] : a[3]), vb = i < 4 ? (i < 2 ? b[0] : b[1]) : (i < 6 ? b[2] : b[3]);
+        x1 = (i & 1) ? va.y : va.x;
+        x2 = (i & 1) ? vb.y : vb.x;
+      }
+      if (kTurn) {
+        const float2 vc = i < 4 ? (i < 2 ? turn.c[0] : turn.c[1]) : (i < 6 ? turn.c[2] : turn.c[3]), vs = i < 4 ? (i < 2 ? turn.s[0] : turn.s[1]) : (i < 6 ? turn.s[2] : turn.s[3]);
+        c = static_cast<double>((i & 1) ? vc.y : vc.x) + static_cast<double>(turn.low[2 * i]);
+        s = static_cast<double>((i & 1) ? vs.y : vs.x) + static_cast<double>(turn.low[2 * i + 1]);
+      }
+      const float y1 = kMagic + code_exact(kTurn ? __dadd_rn(__dmul_rn(x1, c), -__dmul_rn(x2, s)) : x1, scale64);
+      const float y2 = kMagic + code_exact(kTurn ? __dadd_rn(__dmul_rn(x2, c), __dmul_rn(x1, s)) : x2, scale64);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) { ca[i] = kMagic + code_exact(a[i], scale64); cb[i] = kMagic + code_exact(b[i], scale64); }
+      for (int k = 0; k < 4; ++k) {                  // (an index that is known only here would put the codes into memory)
+        if (kTurn && kInterleaved) {
+          if (i == k) code[0][k] = make_float2(y1, y2);
+          if (i == k + 4) code[1][k] = make_float2(y1, y2);
+        } else {
+          if (i == 2 * k) { code[0][k].x = y1; code[1][k].x = y2; }
+          if (i == 2 * k + 1) { code[0][k].y = y1; code[1][k].y = y2; }
+        }
+      }
     }
   }
-  first = pack8(ca);
-  second = pack8(cb);
+  first = pack8(code[0]);
+  second = pack8(code[1]);
 }
 
 // A warp takes some heads of one token, 512 / D at a time; thread l of the D / 16 that share a head has pairs 8 l .. 8 l + 7 of it where it is
-// rotated, elements 16 l .. 16 l + 15 otherwise.
-template <int D, typename T>
+// rotated, elements 16 l .. 16 l + 15 otherwise.  The next head's elements are asked for before this one's are quantised.
+template <int D, typename T, bool kInterleaved>
 __global__ void __launch_bounds__(kThreads) append_kernel(const Params p) {
   constexpr int kLanes = D / 16, kHeads = 32 / kLanes;
   grouped::follow_previous_kernel();
@@ -151,62 +181,63 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const Params p) {
   if (token >= p.tokens) return;
   const int position = p.positions[token];
   long long slot = p.slots != nullptr ? p.slots[token] : 0;
+  const bool turned = 16 * l < p.rot;
+  const int half = p.rot / 2;
+  const int heads = p.H + 2 * p.Hkv;
+  const int head0 = part * p.rounds * kHeads + lane / kLanes, stop = min(heads, head0 + p.rounds * kHeads);
+  Eight<T> a, b, next_a, next_b;
+  auto load = [&](int head, Eight<T>& x, Eight<T>& y) {
+    const int kind = head < p.H ? 0 : head < p.H + p.Hkv ? 1 : 2;
+    const T* in = kind == 0 ? static_cast<const T*>(p.q) + token * p.q_stride + head * D
+                  : kind == 1 ? static_cast<const T*>(p.k) + token * p.k_stride + (head - p.H) * D : static_cast<const T*>(p.v) + token * p.v_stride + (head - p.H - p.Hkv) * D;
+    const bool apart = !kInterleaved && turned && kind != 2;      // halves of the rotated part
+    load8(in + (apart ? 8 * l : 16 * l), x);
+    load8(in + (apart ? half + 8 * l : 16 * l + 8), y);
+  };
+  if (head0 < stop) load(head0, a, b);
   const bool no_position = position < 0 || position >= p.in_table, no_slot = p.slots != nullptr && slot >= p.num_slots;
   if ((no_position || no_slot) && lane == 0 && part == 0) report(p.status, p.host_word, FMHA_I8_DEV_BAD_INDEX, 2u, token);
   if (no_position) return;
   if (no_slot) slot = -1;
-  const bool turned = 16 * l < p.rot;
-  const int half = p.rot / 2;
-  // elements a = [at_a, at_a + 8) and b = [at_b, at_b + 8)
-  const int at_a = turned && !p.interleaved ? 8 * l : 16 * l, at_b = turned && !p.interleaved ? half + 8 * l : 16 * l + 8;
-  float2 cs[8];
-  float most_cs = 1.f;
-  const float* low = nullptr;
+  Turn turn;
+  turn.most = 0.f;
+  turn.low = nullptr;
   if (turned) {
     const float* row = p.table + (static_cast<long long>(position) * half + 8 * l) * 2;
-    low = row + p.in_table * p.rot;
-    most_cs = 0.f;
+    turn.low = row + p.in_table * p.rot;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float4 t = reinterpret_cast<const float4*>(row)[i];
-      cs[2 * i] = make_float2(t.x, t.y);
-      cs[2 * i + 1] = make_float2(t.z, t.w);
-      most_cs = max3_abs(max3_abs(most_cs, t.x, t.y), t.z, t.w);
+      turn.c[i] = make_float2(t.x, t.z);
+      turn.s[i] = make_float2(t.y, t.w);
+      turn.most = max3_abs(max3_abs(turn.most, t.x, t.y), t.z, t.w);
     }
   }
-  const int heads = p.H + 2 * p.Hkv;
-  const int head0 = part * p.rounds * kHeads + lane / kLanes;
 #pragma unroll 1
-  for (int r = 0; r < p.rounds; ++r) {
-    const int head = head0 + r * kHeads;
-    if (head >= heads) break;
+  for (int head = head0; head < stop; head += kHeads) {
+    if (head + kHeads < stop) load(head + kHeads, next_a, next_b);
     const int kind = head < p.H ? 0 : head < p.H + p.Hkv ? 1 : 2;
     const int h = kind == 0 ? head : kind == 1 ? head - p.H : head - p.H - p.Hkv;
-    int8_t* out;
-    if (kind == 0) {
-      out = p.q_out + (static_cast<long long>(token) * p.H + h) * D;
-    } else {
-      out = kind == 1 ? p.k_out : p.v_out;
-      if (p.slots == nullptr) out += (static_cast<long long>(token) * p.Hkv + h) * D;
-      else if (slot >= 0) out += (slot >> p.page_shift) * p.page_stride + ((static_cast<long long>(h) << p.page_shift) + (slot & ((1 << p.page_shift) - 1))) * D;
-      else continue;
+    int8_t* out = kind == 0 ? p.q_out + (static_cast<long long>(token) * p.H + h) * D : kind == 1 ? p.k_out : p.v_out;
+    if (kind != 0)
+      out += p.slots == nullptr ? (static_cast<long long>(token) * p.Hkv + h) * D
+                                : (slot >> p.page_shift) * p.page_stride + ((static_cast<long long>(h) << p.page_shift) + (slot & ((1 << p.page_shift) - 1))) * D;
+    if (kind == 0 || slot >= 0) {
+      float2 x[4], y[4];
+      floats<T>(a, x);
+      floats<T>(b, y);
+      uint2 first, second;
+      if (turned && kind != 2) quantise16<true, kInterleaved>(x, y, turn, p.amax[kind], p.scale[kind], first, second);
+      else quantise16<false, false>(x, y, turn, p.amax[kind], p.scale[kind], first, second);
+      if (!kInterleaved && turned && kind != 2) {
+        *reinterpret_cast<uint2*>(out + 8 * l) = first;
+        *reinterpret_cast<uint2*>(out + half + 8 * l) = second;
+      } else {
+        *reinterpret_cast<uint4*>(out + 16 * l) = make_uint4(first.x, first.y, second.x, second.y);
+      }
     }
-    const T* in = static_cast<const T*>(kind == 0 ? p.q : kind == 1 ? p.k : p.v) + token * (kind == 0 ? p.q_stride : kind == 1 ? p.k_stride : p.v_stride) + h * D;
-    const float amax = p.amax[kind], scale = p.scale[kind];
-    float a[8], b[8];
-    uint2 first, second;
-    if (turned && kind != 2) {
-      Load<T>::eight(in + at_a, a);
-      Load<T>::eight(in + at_b, b);
-      quantise16<true>(a, b, cs, most_cs, low, p.interleaved != 0, amax, scale, first, second);
-      *reinterpret_cast<uint2*>(out + at_a) = first;
-      *reinterpret_cast<uint2*>(out + at_b) = second;
-    } else {
-      Load<T>::eight(in + 16 * l, a);
-      Load<T>::eight(in + 16 * l + 8, b);
-      quantise16<false>(a, b, cs, 1.f, nullptr, false, amax, scale, first, second);
-      *reinterpret_cast<uint4*>(out + 16 * l) = make_uint4(first.x, first.y, second.x, second.y);
-    }
+    a = next_a;
+    b = next_b;
   }
 }
 

@@ -35,7 +35,7 @@ template <int D> struct Cfg {
 template <int D, int W, int kRows> struct Smem {
   alignas(1024) uint8_t ring[2 * W * kTile * D];     // per warp: one K tile, one V tile; at the end its partial rows
   float2 stat[W][kRows];                             // reference exponent and sum of each partial row
-  float weight[kMaxCluster * W][kRows];              // what each partial row counts in the whole
+  float2 together[kRows];                            // the same of the CTA's rows
   uint64_t k_full[W], v_full[W];
   int abort;
 };
@@ -342,38 +342,59 @@ rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
       for (int j = 0; j < kOut; j += 4)
         *reinterpret_cast<float4*>(dst + y * (D / 8) + j) = make_float4(o[h][j][y], o[h][j + 1][y], o[h][j + 2][y], o[h][j + 3][y]);
   }
-  cluster_arrive();
-  cluster_wait();
-
-  // ---- every CTA of the cluster puts together its part of the outputs
-  const int parts = ctas * W;
-  for (int i = threadIdx.x; i < kRows; i += W * 32) {
-    float m = -INFINITY, l = 0.f;
-    for (int y = 0; y < parts; ++y) m = fmaxf(m, ld_cluster_v2(map_to_rank(smem_u32(&sm.stat[y % W][i]), y / W)).x);
-    const float base = m == -INFINITY ? 0.f : m;
-    for (int y = 0; y < parts; ++y) {
-      const float2 st = ld_cluster_v2(map_to_rank(smem_u32(&sm.stat[y % W][i]), y / W));
-      const float e = ex2((st.x - base) * p.c2);
-      l = fmaf(e, st.y, l);
-      sm.weight[y][i] = e;
-    }
-    const float inv = l > 0.f ? p.out_scale / (kEight ? l * kLevels : l) : 0.f;
-    for (int y = 0; y < parts; ++y) sm.weight[y][i] *= inv;
-  }
   __syncthreads();
+
+  // ---- the CTA puts its warps' rows together, then the cluster its CTAs': one thread, four outputs
   constexpr int kQuads = D / 4;
-  for (int i = rank * W * 32 + threadIdx.x; i < kRows * kQuads; i += ctas * W * 32) {
-    const int r = i / kQuads, c = i % kQuads, row = row0 + r;
-    if (row >= n_rows) break;
-    float a[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int y = 0; y < parts; ++y) {
-      const float e = sm.weight[y][r];
-      if (e == 0.f) continue;                        // a warp without keys for this row
-      const float4 v = ld_cluster_v4(map_to_rank(smem_u32(sm.ring + (y % W) * 2 * C::kTileBytes) + static_cast<uint32_t>((r * D + 4 * c) * 4), y / W));
+  auto store = [&](int r, int c, float l, float (&a)[4]) {
+    const int row = row0 + r, token = row / p.G;
+    if (row >= n_rows) return;
+    const float scale = l > 0.f ? p.out_scale / (kEight ? l * kLevels : l) : 0.f;
+#pragma unroll
+    for (int y = 0; y < 4; ++y) a[y] *= scale;
+    store4(p.o, p.o_type, (s.q0 + token) * p.o_stride + static_cast<long long>(head * p.G + row - token * p.G) * D + 4 * c, a);
+  };
+  float* together = reinterpret_cast<float*>(sm.ring + C::kTileBytes);      // behind the first warp's rows
+  for (int i = threadIdx.x; i < kRows * kQuads; i += W * 32) {
+    const int r = i / kQuads, c = i % kQuads;
+    float m = -INFINITY, l = 0.f, a[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int y = 0; y < W; ++y) m = fmaxf(m, sm.stat[y][r].x);
+    const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int y = 0; y < W; ++y) {
+      const float2 st = sm.stat[y][r];
+      const float e = ex2((st.x - base) * p.c2);
+      const float4 v = *reinterpret_cast<const float4*>(sm.ring + y * 2 * C::kTileBytes + (r * D + 4 * c) * 4);
+      l = fmaf(e, st.y, l);
       a[0] = fmaf(e, v.x, a[0]); a[1] = fmaf(e, v.y, a[1]); a[2] = fmaf(e, v.z, a[2]); a[3] = fmaf(e, v.w, a[3]);
     }
-    const int token = row / p.G;
-    store4(p.o, p.o_type, (s.q0 + token) * p.o_stride + static_cast<long long>(head * p.G + row - token * p.G) * D + 4 * c, a);
+    if (ctas == 1) {
+      store(r, c, l, a);
+    } else {
+      *reinterpret_cast<float4*>(together + r * D + 4 * c) = make_float4(a[0], a[1], a[2], a[3]);
+      if (c == 0) sm.together[r] = make_float2(m, l);
+    }
+  }
+  if (ctas == 1) return;
+  cluster_arrive();
+  cluster_wait();
+  const uint32_t rows_at = smem_u32(together), stat_at = smem_u32(sm.together);
+  for (int i = rank * W * 32 + threadIdx.x; i < kRows * kQuads; i += ctas * W * 32) {
+    const int r = i / kQuads, c = i % kQuads;
+    float m = -INFINITY, l = 0.f, a[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int y = 0; y < ctas; ++y) m = fmaxf(m, ld_cluster_v2(map_to_rank(stat_at + 8 * r, y)).x);
+    const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll 4
+    for (int y = 0; y < ctas; ++y) {
+      const float2 st = ld_cluster_v2(map_to_rank(stat_at + 8 * r, y));
+      const float4 v = ld_cluster_v4(map_to_rank(rows_at + static_cast<uint32_t>((r * D + 4 * c) * 4), y));
+      const float e = ex2((st.x - base) * p.c2);
+      l = fmaf(e, st.y, l);
+      a[0] = fmaf(e, v.x, a[0]); a[1] = fmaf(e, v.y, a[1]); a[2] = fmaf(e, v.z, a[2]); a[3] = fmaf(e, v.w, a[3]);
+    }
+    store(r, c, l, a);
   }
   cluster_arrive();                                  // nobody leaves while another still reads its rows
   cluster_wait();

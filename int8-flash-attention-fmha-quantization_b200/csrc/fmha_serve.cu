@@ -197,11 +197,13 @@ template <int D, int kRows> int launch_rows(cudaStream_t stream, const Device& d
   const long long n_tiles = (c.max_k + grouped::kTile - 1) / grouped::kTile;
   if (units > kMostRows / rows::kMaxCluster) return FMHA_I8_ERR_TOO_LARGE;
   const long long resident = 3LL * dev.sm_count;
-  int ctas = 1;
-  while (ctas < 8 && ((units * ctas < 2 * resident && n_tiles >= 4 * ctas * W) || (units * ctas * 2 <= resident && n_tiles >= 2 * ctas * W))) ctas *= 2;
+  // Few units with many keys: one CTA with all the warps of an SM on as many SMs as a cluster allows.
   const int clusters16 = D == 128 ? g_once[dev.index].clusters16_d128 : g_once[dev.index].clusters16_d64;
-  if (ctas == 8 && units <= clusters16 && n_tiles >= 32 * Wide)
-    return launch(rows::rows_kernel<D, Wide, kRows>, static_cast<unsigned>(units * 16), Wide * 32, sizeof(rows::Smem<D, Wide, kRows>), stream, 16u, mk, mv, p);
+  for (const int ctas : {16, 8})
+    if (units * ctas <= dev.sm_count && (ctas == 8 || units <= clusters16) && n_tiles >= 2LL * ctas * Wide)
+      return launch(rows::rows_kernel<D, Wide, kRows>, static_cast<unsigned>(units * ctas), Wide * 32, sizeof(rows::Smem<D, Wide, kRows>), stream, static_cast<unsigned>(ctas), mk, mv, p);
+  int ctas = 1;
+  while (ctas < 8 && ((units * ctas < 2 * resident && n_tiles >= 4 * ctas * W) || (units * ctas * 2 <= resident && n_tiles > ctas * W))) ctas *= 2;
   return launch(rows::rows_kernel<D, W, kRows>, static_cast<unsigned>(units * ctas), W * 32, sizeof(rows::Smem<D, W, kRows>), stream, static_cast<unsigned>(ctas), mk, mv, p);
 }
 
@@ -305,8 +307,10 @@ int rope_table_impl(void* stream, const double* inv_freq, int pairs, long long p
   return cudaGetLastError() == cudaSuccess ? FMHA_I8_OK : FMHA_I8_ERR_LAUNCH;
 }
 
-template <typename T> int launch_append(cudaStream_t stream, const rope::Params& p, int D, unsigned grid) {
-  return D == 128 ? launch(rope::append_kernel<128, T>, grid, rope::kThreads, 0, stream, 0u, p) : launch(rope::append_kernel<64, T>, grid, rope::kThreads, 0, stream, 0u, p);
+template <typename T> int launch_append(cudaStream_t stream, const rope::Params& p, int D, bool interleaved, unsigned grid) {
+  auto* fn = D == 128 ? (interleaved ? rope::append_kernel<128, T, true> : rope::append_kernel<128, T, false>)
+                      : (interleaved ? rope::append_kernel<64, T, true> : rope::append_kernel<64, T, false>);
+  return launch(fn, grid, rope::kThreads, 0, stream, 0u, p);
 }
 
 int append_impl(void* stream, const float amax[5], const long long dims[5], const void* q, const void* k, const void* v, int in_type, const long long strides[3],
@@ -345,7 +349,6 @@ int append_impl(void* stream, const float amax[5], const long long dims[5], cons
   p.H = static_cast<int>(H);
   p.Hkv = static_cast<int>(Hkv);
   p.rot = static_cast<int>(rot);
-  p.interleaved = interleaved != 0;
   for (int i = 0; i < 3; ++i) { p.amax[i] = amax[i]; p.scale[i] = 127.f / amax[i]; }
   Device dev;
   int st = fmha_host::device_for_call(&dev);
@@ -360,9 +363,9 @@ int append_impl(void* stream, const float amax[5], const long long dims[5], cons
   const long long blocks = (tokens * p.parts + rope::kThreads / 32 - 1) / (rope::kThreads / 32);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const unsigned grid = static_cast<unsigned>(blocks);
-  if (in_type == FMHA_I8_TYPE_BF16) return launch_append<__nv_bfloat16>(s, p, static_cast<int>(D), grid);
-  if (in_type == FMHA_I8_TYPE_FP16) return launch_append<__half>(s, p, static_cast<int>(D), grid);
-  return launch_append<float>(s, p, static_cast<int>(D), grid);
+  if (in_type == FMHA_I8_TYPE_BF16) return launch_append<__nv_bfloat16>(s, p, static_cast<int>(D), interleaved != 0, grid);
+  if (in_type == FMHA_I8_TYPE_FP16) return launch_append<__half>(s, p, static_cast<int>(D), interleaved != 0, grid);
+  return launch_append<float>(s, p, static_cast<int>(D), interleaved != 0, grid);
 }
 
 }  // namespace
