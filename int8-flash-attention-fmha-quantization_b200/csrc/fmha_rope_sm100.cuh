@@ -15,7 +15,7 @@ namespace rope {
 using grouped::kMagic;
 using grouped::report;
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 
 struct Params {
   const void *q, *k, *v;
@@ -135,33 +135,29 @@ __device__ __forceinline__ void quantise16(float2 (&a)[4], float2 (&b)[4], const
   // (beyond 2^22 a float next to kMagic has no room for n; d is then as large as z or not a number)
   if (!(off < 0.5f - error)) {
     const double scale64 = 127.0 / static_cast<double>(amax);
-#pragma unroll 1
-    for (int i = 0; i < 8; ++i) {
-      double x1, x2, c = 1.0, s = 0.0;
-      if (kTurn && kInterleaved) {
-        const float2 v = i < 4 ? (i < 2 ? (i == 0 ? a[0] : a[1]) : (i == 2 ? a[2] : a[3])) : (i < 6 ? (i == 4 ? b[0] : b[1]) : (i == 6 ? b[2] : b[3]));
-        x1 = v.x; x2 = v.y;
-      } else {
-        const float2 va = i < 4 ? (i < 2 ? a[0] : a[1]) : (i < 6 ? a[2] : a[3]), vb = i < 4 ? (i < 2 ? b[0] : b[1]) : (i < 6 ? b[2] : b[3]);
-        x1 = (i & 1) ? va.y : va.x;
-        x2 = (i & 1) ? vb.y : vb.x;
-      }
-      if (kTurn) {
-        const float2 vc = i < 4 ? (i < 2 ? turn.c[0] : turn.c[1]) : (i < 6 ? turn.c[2] : turn.c[3]), vs = i < 4 ? (i < 2 ? turn.s[0] : turn.s[1]) : (i < 6 ? turn.s[2] : turn.s[3]);
-        c = static_cast<double>((i & 1) ? vc.y : vc.x) + static_cast<double>(turn.low[2 * i]);
-        s = static_cast<double>((i & 1) ? vs.y : vs.x) + static_cast<double>(turn.low[2 * i + 1]);
-      }
-      const float y1 = kMagic + code_exact(kTurn ? __dadd_rn(__dmul_rn(x1, c), -__dmul_rn(x2, s)) : x1, scale64);
-      const float y2 = kMagic + code_exact(kTurn ? __dadd_rn(__dmul_rn(x2, c), __dmul_rn(x1, s)) : x2, scale64);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {                  // (an index that is known only here would put the codes into memory)
-        if (kTurn && kInterleaved) {
-          if (i == k) code[0][k] = make_float2(y1, y2);
-          if (i == k + 4) code[1][k] = make_float2(y1, y2);
-        } else {
-          if (i == 2 * k) { code[0][k].x = y1; code[1][k].x = y2; }
-          if (i == 2 * k + 1) { code[0][k].y = y1; code[1][k].y = y2; }
-        }
+    for (int i = 0; i < 8; ++i) {
+      const float2 v = i < 4 ? a[i & 3] : b[i & 3];
+      const float x1 = kTurn && kInterleaved ? v.x : at(a, i), x2 = kTurn && kInterleaved ? v.y : at(b, i);
+      const float c = kTurn ? at(turn.c, i) : 1.f, s = kTurn ? at(turn.s, i) : 0.f;
+      // which of the pairs it is: the same as above, within the error
+      const float z1 = fmaf(x1, c, -(x2 * s)) * scale, z2 = fmaf(x2, c, x1 * s) * scale;
+      const float d = fmaxf(fabsf(z1 - rintf(z1)), fabsf(z2 - rintf(z2)));
+      if (d < 0.5f - 2.f * error) continue;
+      double c64 = 1.0, s64 = 0.0;
+      if (kTurn) {
+        c64 = static_cast<double>(c) + static_cast<double>(turn.low[2 * i]);
+        s64 = static_cast<double>(s) + static_cast<double>(turn.low[2 * i + 1]);
+      }
+      const double u1 = x1, u2 = x2;
+      const float y1 = kMagic + code_exact(kTurn ? __dadd_rn(__dmul_rn(u1, c64), -__dmul_rn(u2, s64)) : u1, scale64);
+      const float y2 = kMagic + code_exact(kTurn ? __dadd_rn(__dmul_rn(u2, c64), __dmul_rn(u1, s64)) : u2, scale64);
+      if (kTurn && kInterleaved) {
+        code[i >> 2][i & 3] = make_float2(y1, y2);
+      } else if (i & 1) {
+        code[0][i >> 1].y = y1; code[1][i >> 1].y = y2;
+      } else {
+        code[0][i >> 1].x = y1; code[1][i >> 1].x = y2;
       }
     }
   }
@@ -172,7 +168,7 @@ __device__ __forceinline__ void quantise16(float2 (&a)[4], float2 (&b)[4], const
 // A warp takes some heads of one token, 512 / D at a time; thread l of the D / 16 that share a head has pairs 8 l .. 8 l + 7 of it where it is
 // rotated, elements 16 l .. 16 l + 15 otherwise.  The next head's elements are asked for before this one's are quantised.
 template <int D, typename T, bool kInterleaved>
-__global__ void __launch_bounds__(kThreads) append_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, 5) append_kernel(const Params p) {
   constexpr int kLanes = D / 16, kHeads = 32 / kLanes;
   grouped::follow_previous_kernel();
   const int lane = threadIdx.x & 31, l = lane % kLanes;
