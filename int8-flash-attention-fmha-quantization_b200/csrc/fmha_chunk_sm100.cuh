@@ -54,6 +54,7 @@ struct Unit : Steps {
   int b, head;
   int token0;           // first token of tile A; tile B begins tq later
   int end;              // keys that the last token of the unit sees
+  int first;            // key tile at which this CTA begins (0 unless the unit is split)
 };
 template <int D> struct Ctl {
   using C = Cfg<D>;
@@ -65,7 +66,11 @@ template <int D> struct Ctl {
   uint32_t tmem_base;
   int abort;
   Unit unit[kInfos];
+  float2 part[2][kTile];                             // split units: a row's reference and sum in this CTA
 };
+// Split units: where a CTA leaves its rows for the others once its tiles are no longer needed, four floats further apart than they are long.
+template <int D> constexpr int kPitch = D + 4;
+static_assert(2 * kTile * kPitch<128> * 4 <= Cfg<128>::kBias - Cfg<128>::kK && 2 * kTile * kPitch<64> * 4 <= Cfg<64>::kBias - Cfg<64>::kK, "the partial rows do not fit");
 template <int D> constexpr size_t smem_bytes() { return 1024 + Cfg<D>::kBytes + sizeof(Ctl<D>); }
 
 // Reads units in order, one slot of the ring after the other.
@@ -111,7 +116,7 @@ struct Failure {
 // ------------------------------------------------------------------------------------------------ units
 // The pairs of tiles of all sequences, the last of each sequence first, then the ones before those, and so on: with causal masks the ones with most keys
 // come first.  Every pair is one unit per key head.  CTA c takes units c, 2 grid - 1 - c, 2 grid + c, ...: a round in one direction, the next in the other.
-template <int D> __device__ __forceinline__ void walk_role(const Params& p, Ctl<D>* ctl) {
+template <int D, bool kSplit> __device__ __forceinline__ void walk_role(const Params& p, Ctl<D>* ctl) {
   const int lane = threadIdx.x & 31;
   const Failure fail{p, &ctl->abort};
   int level = -1, before = 0, here = 0;             // pairs of earlier levels, and of this one
@@ -125,11 +130,11 @@ template <int D> __device__ __forceinline__ void walk_role(const Params& p, Ctl<
   const int few = p.B <= 32 ? pairs_of(lane) : 0;   // up to 32 sequences: kept in registers
   for (uint32_t n = 0;; ++n) {
     const long long round = n, ctas = gridDim.x;
-    const long long u = round * ctas + ((n & 1u) ? ctas - 1 - blockIdx.x : blockIdx.x);
+    const long long u = kSplit ? static_cast<long long>(blockIdx.x / cluster_ctas()) : round * ctas + ((n & 1u) ? ctas - 1 - blockIdx.x : blockIdx.x);
     const int head = static_cast<int>(u % p.Hkv);
     const long long pair = u / p.Hkv;
-    bool more = true;
-    while (level < 0 || pair >= static_cast<long long>(before) + here) {
+    bool more = !kSplit || n == 0;
+    while (more && (level < 0 || pair >= static_cast<long long>(before) + here)) {
       before += here;
       ++level;
       here = 0;
@@ -165,6 +170,13 @@ template <int D> __device__ __forceinline__ void walk_role(const Params& p, Ctl<
         const int keys = first < unit.seq.nq ? visible(p, unit.seq, last) : 0;
         unit.n[t] = (keys + kTile - 1) / kTile;
         unit.end = max(unit.end, keys);
+      }
+      if constexpr (kSplit) {
+        const int all = unit.all(), parts = static_cast<int>(cluster_ctas()), rank = static_cast<int>(cluster_rank());
+        unit.first = static_cast<int>(static_cast<long long>(all) * rank / parts);
+        const int last = static_cast<int>(static_cast<long long>(all) * (rank + 1) / parts);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) unit.n[t] = max(min(unit.n[t], last) - unit.first, 0);
       }
     }
     const uint32_t slot = n % kInfos;
@@ -204,12 +216,12 @@ template <int D> __device__ __forceinline__ void load_role(const Params& p, Ctl<
     }
     __syncwarp();
     ++nq;
-    int page = page_of(p, u.b, 0, u.end, lane);
+    int page = page_of(p, u.b, u.first * kTile, u.end, lane);
     for (int j = 0; j < n; ++j, ++g) {
-      const int copies = copies_of(p, j * kTile, u.end);
+      const int key0 = (u.first + j) * kTile, copies = copies_of(p, key0, u.end);
       const uint32_t bytes = static_cast<uint32_t>((copies << p.box_shift) * D);
       if (page < 0 || page >= p.num_pages) { page = p.num_pages; bad_page |= lane < copies; }      // reads zeros
-      const int next_page = page_of(p, u.b, (j + 1) * kTile, u.end, lane);
+      const int next_page = page_of(p, u.b, key0 + kTile, u.end, lane);
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv) {
         const uint32_t stages = kv ? C::kStagesV : C::kStagesK, st = g % stages;
@@ -217,7 +229,7 @@ template <int D> __device__ __forceinline__ void load_role(const Params& p, Ctl<
         if (g >= stages && !warp_wait(empty, ((g / stages) - 1) & 1u, abort_flag)) return fail(kv ? FMHA_I8_DEV_WAIT_V_FREE : FMHA_I8_DEV_WAIT_K_FREE, g);
         if (lane == 0) mbar_arrive_expect_tx(full, bytes);
         __syncwarp();
-        if (lane < copies) issue_copy<D>(p, kv ? map_v : map_k, smem + (kv ? C::kV : C::kK) + st * C::kTileBytes, full, u.seq, u.head, j * kTile, lane, page);
+        if (lane < copies) issue_copy<D>(p, kv ? map_v : map_k, smem + (kv ? C::kV : C::kK) + st * C::kTileBytes, full, u.seq, u.head, key0, lane, page);
         __syncwarp();
       }
       page = next_page;
@@ -408,7 +420,7 @@ template <int D> __device__ __forceinline__ void output_role(const Params& p, Ct
 // ------------------------------------------------------------------------------------------------ softmax
 __device__ __forceinline__ int max3(int a, int b, int c) { return __vimax3_s32(a, b, c); }
 
-template <int D, bool kWide> __device__ __forceinline__ void softmax_role(const Params& p, Ctl<D>* ctl, uint32_t tmem) {
+template <int D, bool kWide, bool kSplit> __device__ __forceinline__ void softmax_role(const Params& p, Ctl<D>* ctl, uint32_t tmem) {
   const int warp = warp_index(), t = warp >> 2, quad = warp & 3, lane = threadIdx.x & 31;
   const int row = quad * 32 + lane;
   const Failure fail{p, &ctl->abort};
@@ -429,10 +441,10 @@ template <int D, bool kWide> __device__ __forceinline__ void softmax_role(const 
     {
       const int token = u.token0 + t * p.tq + my_token;
       real = my_token < p.tq && token < u.seq.nq;
-      limit = real ? visible(p, u.seq, token) : 0;
+      limit = (real ? visible(p, u.seq, token) : 0) - (kSplit ? u.first * kTile : 0);      // (of this CTA's keys)
     }
     const bool any = __any_sync(0xFFFFFFFFu, limit > 0);            // a warp without a row that sees a key leaves its part of P as it is
-    const int least = __reduce_min_sync(0xFFFFFFFFu, real ? limit : 0x7FFFFFFF);
+    const int least = __reduce_min_sync(0xFFFFFFFFu, real ? limit : 0x7FFFFFFF);      // keys that all rows see
     // p = 2^((x - ref) c2), x and ref as the floats kMagic + score.  Exponents are x c2 - hi with hi = ref c2 rounded, the same for a row as long as its
     // reference is, and rounded once.  Where c2 is large the difference is taken first: hi would be off by as much as 16.
     int ref = 0;
@@ -529,6 +541,14 @@ template <int D, bool kWide> __device__ __forceinline__ void softmax_role(const 
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&ctl->p_ready[t][1]));
     }
+    if constexpr (kSplit) {                          // the rows are put together behind all roles
+      if (n > 0 && !warp_wait(smem_u32(&ctl->o_full[t]), outs & 1u, abort_flag)) return fail(FMHA_I8_DEV_WAIT_O_READY, steps);
+      if (n > 0) ++outs;
+      const float l = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+      ctl->part[t][row] = make_float2(__int_as_float(ref), n > 0 && limit > 0 ? l : 0.f);
+      units.release();
+      continue;
+    }
     // ---- the row's output
     const long long at = (u.seq.q0 + u.token0 + t * p.tq + my_token) * p.o_stride + static_cast<long long>((u.head - my_token) * p.G + row) * D;
     units.release();
@@ -562,8 +582,66 @@ template <int D, bool kWide> __device__ __forceinline__ void softmax_role(const 
   }
 }
 
-// kWide: the factor from scores to exponents is large (see softmax_role).
-template <int D, bool kWide>
+// The parts of a split unit: every CTA leaves its rows, references and sums in shared memory, and puts together its share of them.  By all threads.
+template <int D> __device__ __forceinline__ void join_parts(const Params& p, Ctl<D>* ctl, uint8_t* tiles, uint32_t tmem) {
+  const int warp = warp_index(), lane = threadIdx.x & 31;
+  const int parts = static_cast<int>(cluster_ctas()), rank = static_cast<int>(cluster_rank());
+  const Unit& u = ctl->unit[0];
+  float* rows = reinterpret_cast<float*>(tiles + Cfg<D>::kK);
+  if (warp < kWarpConvert && u.valid) {
+    const int t = warp >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t tO = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + 2 * kTile + t * kTile;
+    const bool some = ctl->part[t][row].y > 0.f;
+    if (__any_sync(0xFFFFFFFFu, some)) {
+#pragma unroll 1
+      for (int i = 0; i < D; i += 16) {
+        uint32_t o[16];
+        tmem_ld16_issue(tO + i, o);
+        tmem_ld_fence(o);
+        float4* to = reinterpret_cast<float4*>(rows + (t * kTile + row) * kPitch<D> + i);
+#pragma unroll
+        for (int y = 0; y < 4; ++y) to[y] = make_float4(__uint_as_float(o[4 * y]), __uint_as_float(o[4 * y + 1]), __uint_as_float(o[4 * y + 2]), __uint_as_float(o[4 * y + 3]));
+      }
+    }
+  }
+  __syncwarp();
+  cluster_arrive();
+  cluster_wait();
+  if (u.valid) {
+    constexpr int kQuads = D / 4;
+    const uint32_t rows_at = smem_u32(rows), part_at = smem_u32(ctl->part);
+    const int from = 2 * kTile * rank / parts, to = 2 * kTile * (rank + 1) / parts;
+    for (int i = from * kQuads + static_cast<int>(threadIdx.x); i < to * kQuads; i += kThreads) {
+      const int r = i / kQuads, c = i - r * kQuads, t = r / kTile, in_tile = r - t * kTile, my_token = in_tile / p.G;
+      const int token = u.token0 + t * p.tq + my_token;
+      if (my_token >= p.tq || token >= u.seq.nq) continue;
+      float m = 0.f, l = 0.f, a[4] = {0.f, 0.f, 0.f, 0.f};           // (references are floats above 2^22)
+      for (int y = 0; y < parts; ++y) {
+        const float2 st = ld_cluster_v2(map_to_rank(part_at + 8 * r, y));
+        if (st.y > 0.f) m = fmaxf(m, st.x);
+      }
+      for (int y = 0; y < parts; ++y) {
+        const float2 st = ld_cluster_v2(map_to_rank(part_at + 8 * r, y));
+        if (!(st.y > 0.f)) continue;
+        const float e = ex2((st.x - m) * p.c2);
+        const float4 v = ld_cluster_v4(map_to_rank(rows_at + static_cast<uint32_t>((r * kPitch<D> + 4 * c) * 4), y));
+        l = fmaf(e, st.y, l);
+        a[0] = fmaf(e, v.x, a[0]); a[1] = fmaf(e, v.y, a[1]); a[2] = fmaf(e, v.z, a[2]); a[3] = fmaf(e, v.w, a[3]);
+      }
+      const float scale = l > 0.f ? p.out_scale / l : 0.f;
+#pragma unroll
+      for (int y = 0; y < 4; ++y) a[y] *= scale;
+      store4(p.o, p.o_type, (u.seq.q0 + token) * p.o_stride + static_cast<long long>(u.head * p.G + in_tile - my_token * p.G) * D + 4 * c, a);
+    }
+  }
+  __syncwarp();
+  cluster_arrive();                                  // nobody leaves while another still reads its rows
+  cluster_wait();
+}
+
+// kWide: the factor from scores to exponents is large (see softmax_role).  kSplit: one unit per cluster, whose CTAs share its key tiles: for calls of few
+// tokens against many keys, whose units would leave most SMs idle.
+template <int D, bool kWide, bool kSplit>
 __global__ void __launch_bounds__(kThreads, 1)
 chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Params p) {
   using C = Cfg<D>;
@@ -608,7 +686,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
 
   if (warp < kWarpConvert) {
     setmaxnreg_inc<kSoftmaxRegs>();
-    softmax_role<D, kWide>(p, ctl, tmem);
+    softmax_role<D, kWide, kSplit>(p, ctl, tmem);
   } else if (warp < kWarpLoad) {
     setmaxnreg_dec<kConvertRegs>();
     convert_role<D>(p, ctl, tiles);
@@ -617,7 +695,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     if (warp == kWarpLoad) load_role<D>(p, ctl, &map_q, &map_k, &map_v, smem_u32(tiles));
     else if (warp == kWarpScore) score_role<D>(p, ctl, smem_u32(tiles), tmem);
     else if (warp == kWarpOutput) output_role<D>(p, ctl, smem_u32(tiles), tmem);
-    else walk_role<D>(p, ctl);
+    else walk_role<D, kSplit>(p, ctl);
   }
   __syncwarp();
   if (ctl->abort) {                                  // copies still in flight land before their memory is used again
@@ -626,6 +704,15 @@ chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (kSplit) {
+    // (the registers as they were at launch again)
+    if (warp < kWarpConvert) setmaxnreg_dec<kLaunchRegs>();
+    else setmaxnreg_inc<kLaunchRegs>();
+    tc_fence_after();
+    join_parts<D>(p, ctl, tiles, tmem);
+    tc_fence_before();
+    __syncthreads();
+  }
   if (warp == 0) {
     tc_fence_after();
     tmem_dealloc(tmem, kTmemCols);

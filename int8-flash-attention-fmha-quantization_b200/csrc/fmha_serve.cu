@@ -95,7 +95,8 @@ template <int D> int count_clusters() {
 }
 
 template <int D> int set_up_chunk() {
-  for (const void* fn : {reinterpret_cast<const void*>(&chunk::chunk_kernel<D, false>), reinterpret_cast<const void*>(&chunk::chunk_kernel<D, true>)}) {
+  for (const void* fn : {reinterpret_cast<const void*>(&chunk::chunk_kernel<D, false, false>), reinterpret_cast<const void*>(&chunk::chunk_kernel<D, true, false>),
+                         reinterpret_cast<const void*>(&chunk::chunk_kernel<D, true, true>)}) {
     cudaFuncAttributes fa{};
     if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(chunk::smem_bytes<D>())) != cudaSuccess ||
         cudaFuncGetAttributes(&fa, fn) != cudaSuccess) {
@@ -211,6 +212,17 @@ template <int D, int kRows> int launch_rows(cudaStream_t stream, const Device& d
 constexpr int kMostGroup = 128;
 bool few_rows(const grouped::Params& p) { return p.G > kMostGroup || static_cast<long long>(p.max_q) * p.G <= 16; }
 
+// CTAs that share a unit of the chunk kernel, in steps of one key tile (1.8 us): a CTA's share of them, and 4 for what a part costs besides.
+int chunk_parts(long long units, long long n_tiles, int sms) {
+  long long best = (units + sms - 1) / sms * (n_tiles + 2);
+  int parts = 1;
+  for (const int c : {2, 4, 8}) {
+    const long long rounds = (units * c + sms - 1) / sms, cost = rounds * ((n_tiles + c - 1) / c + 4);
+    if (cost < best) { best = cost; parts = c; }
+  }
+  return parts;
+}
+
 template <int D> int launch_chunk(cudaStream_t stream, const Device& dev, Call& c, const CUtensorMap& mk, const CUtensorMap& mv) {
   grouped::Params& p = c.p;
   p.tq = grouped::kTile / p.G;
@@ -226,7 +238,10 @@ template <int D> int launch_chunk(cudaStream_t stream, const Device& dev, Call& 
   const long long units = std::min<long long>(p.total_q, p.total_q / (2LL * p.tq) + p.B) * p.Hkv;
   if (units > kMostRows) return FMHA_I8_ERR_TOO_LARGE;
   const unsigned grid = static_cast<unsigned>(std::min<long long>(units, dev.sm_count));
-  return launch(p.c2 > 0.5f ? chunk::chunk_kernel<D, true> : chunk::chunk_kernel<D, false>, grid, chunk::kThreads, chunk::smem_bytes<D>(), stream, 0u, mq, mk, mv, p);
+  const int parts = chunk_parts(units, (c.max_k + grouped::kTile - 1) / grouped::kTile, dev.sm_count);
+  if (parts > 1)
+    return launch(chunk::chunk_kernel<D, true, true>, static_cast<unsigned>(units * parts), chunk::kThreads, chunk::smem_bytes<D>(), stream, static_cast<unsigned>(parts), mq, mk, mv, p);
+  return launch(p.c2 > 0.5f ? chunk::chunk_kernel<D, true, false> : chunk::chunk_kernel<D, false, false>, grid, chunk::kThreads, chunk::smem_bytes<D>(), stream, 0u, mq, mk, mv, p);
 }
 
 int run_attention(void* stream, Call& c) {
