@@ -217,9 +217,53 @@ def test_packed_views_of_a_fused_projection_and_generous_bounds(pkg, torch):
     run_packed(pkg, torch, [100, 260, 9], None, 6, 2, 64, True, "bf16", seed=3, fused=True, max_k=0)
 
 
+def test_more_sequences_than_a_warp_has_lanes(pkg, torch):
+    lens = [(37 * i) % 150 for i in range(75)]
+    run_packed(pkg, torch, lens, None, 4, 2, 64, True, "bf16", seed=1)
+    run_packed(pkg, torch, [300] * 33, None, 8, 2, 128, True, "bf16", seed=2)
+    run_paged(pkg, torch, [1 + i % 40 for i in range(70)], [60 + 3 * i for i in range(70)], 6, 2, 64, 16, "bf16", seed=3)
+    run_paged(pkg, torch, [1] * 150, [1 + (61 * i) % 500 for i in range(150)], 8, 2, 128, 16, "fp16", seed=4)
+
+
+@pytest.mark.parametrize("out", ["bf16", "int8"])
+def test_outputs_with_strides_and_the_least_alignment(pkg, torch, out):
+    """o as a view with a row of its own spacing, 16-byte aligned only: the narrow stores, and nothing besides the rows is touched."""
+    T, H, Hkv, D = 150, 6, 2, 64
+    size = TYPES[out].itemsize
+    q, k, v = codes((T, H, D), 1), codes((T, Hkv, D), 2), codes((T, Hkv, D), 3)
+    flat = torch.full(((T + 1) * (H * D + 16 // size) + 64,), FILL[out], dtype=TYPES[out], device="cuda")
+    o = flat[16 // size:].as_strided((T, H, D), (H * D + 16 // size, D, 1))
+    assert o.data_ptr() % 32 == 16
+    cu = starts([T])
+    for tokens in (T, 1):
+        before = flat.clone()
+        desc = pkg.AttnDataDescriptorGrouped(1, tokens, T, H, Hkv, D)
+        pkg.FMHAInferI8Packed(None, param(pkg), desc, q[:tokens], k, v, starts([tokens]), cu, o[:tokens])
+        want, scales = attention64(q[:tokens], k, v, AMAX, True)
+        check(o[:tokens], want, scales, T, out, AMAX, O_AMAX, tokens * 3)
+        o[:tokens] = FILL[out] if tokens == T else before.as_strided((T, H, D), o.stride(), o.storage_offset())[:tokens]
+        assert torch.equal(flat, before)
+
+
+def test_no_tokens_and_no_keys(pkg, torch):
+    """Calls in which nothing, or nothing but zeros, is to be written."""
+    for D, H in ((64, 4), (128, 48)):                        # few rows, and more than sixteen
+        desc = pkg.AttnDataDescriptorGrouped(2, 5, 5, H, 2, D)
+        empty_k = codes((0, 2, D), 1)
+        o = torch.full((5, H, D), 7.0, dtype=torch.bfloat16, device="cuda")
+        pkg.FMHAInferI8Packed(None, param(pkg), desc, codes((5, H, D), 1), empty_k, empty_k, starts([2, 3]), starts([0, 0]), o)
+        assert not bool(o.any())
+        pkg.FMHAInferI8Packed(None, param(pkg), desc, codes((0, H, D), 1), empty_k, empty_k, starts([0, 0]), starts([0, 0]), o[:0])
+        o.fill_(7.0)
+        kc = codes((1, 2, 16, D), 2)
+        lens = torch.zeros(2, dtype=torch.int32, device="cuda")
+        pkg.FMHAInferI8Paged(None, param(pkg), desc, codes((5, H, D), 1), kc, kc, torch.zeros((2, 1), dtype=torch.int32, device="cuda"), lens, starts([1, 0]), o)
+        assert not bool(o[0].any()) and bool((o[1:] == 7.0).all())
+
+
 def test_packed_rows_that_are_far_from_even(pkg, torch):
     """Ranges so wide that a row's largest score takes everything, and so narrow that all keys count the same."""
-    for a in (1e-9, 40.0, 1e9):
+    for a in (1e-9, 40.0, 250.0, 777.7, 1500.0, 1e9):
         amax = (a, a, AMAX[2])
         q, k, v = codes((150, 4, 64), 1), codes((150, 2, 64), 2), codes((150, 2, 64), 3)
         o = torch.empty((150, 4, 64), dtype=torch.bfloat16, device="cuda")
@@ -227,6 +271,11 @@ def test_packed_rows_that_are_far_from_even(pkg, torch):
         pkg.FMHAInferI8Packed(None, pkg.FMHAParamI8(*amax, 1.0, 1.0), pkg.AttnDataDescriptorGrouped(1, 150, 150, 4, 2, 64), q, k, v, cu, cu, o)
         want, spread = attention64(q, k, v, amax, True)
         check(o, want, spread, 150, "bf16", amax, 1.0, 300, str(a))
+        for tokens in (1, 8):                                # eight rows, and sixteen
+            one = starts([tokens])
+            pkg.FMHAInferI8Packed(None, pkg.FMHAParamI8(*amax, 1.0, 1.0), pkg.AttnDataDescriptorGrouped(1, tokens, 150, 4, 2, 64), q[:tokens], k, v, one, cu, o[:tokens])
+            want, spread = attention64(q[:tokens], k, v, amax, True)
+            check(o[:tokens], want, spread, 150, "bf16", amax, 1.0, 2 * tokens, f"{a}, {tokens}")
 
 
 def test_packed_identical_scores_and_growing_maxima(pkg, torch):
@@ -326,6 +375,10 @@ PAGED = [
     ([5], [3], 6, 2, 64, 16, "bf16"),
     ([520, 1, 1], [1300, 7, 513], 16, 2, 64, 4096, "bf16"),
     ([1, 1], [9000, 8999], 40, 1, 64, 16, "bf16"),
+    ([3, 1], [700, 2000], 10, 2, 128, 16, "fp16"),
+    ([7], [30001], 24, 3, 64, 32, "bf16"),
+    ([40, 2], [9001, 5], 8, 4, 128, 16, "fp16"),
+    ([100], [70000], 2, 1, 128, 64, "bf16"),
 ]
 
 
@@ -339,6 +392,17 @@ def test_paged_other_forms(pkg, torch):
     run_paged(pkg, torch, [1, 50, 1], [333, 444, 5], 6, 3, 64, 32, "bf16", seed=2, causal=False)
     run_paged(pkg, torch, [1, 1, 1], [333, 444, 5], 6, 3, 64, 32, "bf16", seed=3, wide=500, max_k=16000)     # bounds far beyond the lengths
     run_paged(pkg, torch, [1, 1, 1], [3330, 4440, 5], 6, 3, 128, 32, "bf16", seed=4, max_k=1)                  # and far below
+
+
+def test_paged_many_keys_for_one_warp(pkg, torch):
+    """A bound far below the length leaves one CTA to go through all keys: the whole-number sums of a warp fill up more than once."""
+    D, page, n = 128, 4096, 300000
+    kc, vc = codes((3, 1, page, D), 1), codes((3, 1, page, D), 2)
+    table = (torch.arange(-(-n // page), device="cuda") % 3).to(torch.int32)[None].contiguous()      # the same pages over and over
+    q, o = codes((1, 4, D), 3), torch.empty((1, 4, D), dtype=torch.float16, device="cuda")
+    pkg.FMHAInferI8Paged(None, param(pkg), pkg.AttnDataDescriptorGrouped(1, 1, 1, 4, 1, D), q, kc, vc, table, torch.tensor([n], dtype=torch.int32, device="cuda"), starts([1]), o)
+    want, scales = attention64(q, keys_of(kc, table, 0, n), keys_of(vc, table, 0, n), AMAX, True)
+    check(o, want, scales, n, "fp16", AMAX, 1.0, 4)
 
 
 def test_paged_pages_and_lengths_outside_are_reported(pkg, torch):
@@ -480,3 +544,42 @@ def test_calls_on_two_streams_at_once_and_in_a_row(pkg, torch):
         n = 700 + 3 + 260
         for x in out:
             assert torch.equal(x[:n], o[:n])
+
+
+def test_host_threads_call_at_once(pkg, torch):
+    """Four host threads, each with a stream, shapes and a cache of its own."""
+    import threading
+    failures = []
+
+    def work(i):
+        try:
+            torch.cuda.set_device(0)
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for rep in range(5):
+                    run_paged(pkg, torch, [1, 20 * i, 3], [100 + i, 400, 3], 4 * (i + 1), 2, (64, 128)[i % 2], 16, "bf16", seed=10 * i + rep)
+                    run_packed(pkg, torch, [50 * i + 1, 7], None, 4, 2, (128, 64)[i % 2], True, "bf16", seed=rep)
+        except BaseException as e:  # noqa: BLE001
+            failures.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures, failures[0]
+
+
+def test_plain_calls_give_the_same_bytes_every_time(pkg, torch):
+    q, k, v, o = run_packed(pkg, torch, [700, 300], None, 8, 2, 128, True, "bf16", seed=4)
+    kc, vc, table, lens = make_cache(torch, [5000, 900], 2, 128, 16, 4)
+    table.clamp_(min=0)
+    cu = starts([700, 300])
+    first = None
+    for _ in range(5):
+        again = torch.empty_like(o)
+        pkg.FMHAInferI8Packed(None, param(pkg), pkg.AttnDataDescriptorGrouped(2, 700, 700, 8, 2, 128), q, k, v, cu, cu, again)
+        assert torch.equal(again[:1000], o[:1000])
+        one = torch.empty((2, 8, 128), dtype=torch.bfloat16, device="cuda")
+        pkg.FMHAInferI8Paged(None, param(pkg), pkg.AttnDataDescriptorGrouped(2, 1, 5000, 8, 2, 128), q[:2], kc, vc, table, lens, starts([1, 1]), one)
+        first = one if first is None else first
+        assert torch.equal(one, first)
