@@ -2,10 +2,15 @@
 //
 //   y = rotate(x, position),  code = clamp(floor(y * (127 / amax) + 1/2), -127, 127)
 //
-// Bound by memory: every element is read once (2 bytes, or 4) and leaves one byte; the rotation is two multiplications an element.  The codes are
+// Every element is read once (2 bytes, or 4) and leaves one byte; the rotation is two multiplications an element.  The codes are
 // those of 64-bit arithmetic, so that they depend on nothing but their inputs: they are computed in 32 bits, with a bound of the error, and a
-// thread one of whose values lies closer to a border between two codes than that computes its values again in 64 bits, with the table's second
-// plane.  With normal values that is one thread in 600.
+// thread one of whose values lies closer to a border between two codes than that looks for it and computes the pair again in 64 bits, with the table's second
+// plane.  With normal values and ranges of 3 to 5 that is one thread in 600 to 1100 where they are rotated, and one in 30 to 120 where bf16 values are not: their products
+// with the scale reach exact halves.
+//
+// 8192 tokens of 48 heads of 128, bf16: 42 us, 3.7 TB/s, 57 % of a copy's rate.  Issue bounds it (57 % of the cycles, 245 instructions of a warp for 512 elements, 4.3 warps
+// to a scheduler): pairs of values in one instruction, the next head's loads ahead and the search of the one pair made 76 us 42.  A range of v whose halves are not reached
+// (3.93 for 4.25) takes 40.6; the division 127 / range taken out of the 64-bit path changes nothing.
 #pragma once
 #include "fmha_grouped_sm100.cuh"
 

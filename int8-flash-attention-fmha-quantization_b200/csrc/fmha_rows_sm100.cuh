@@ -10,11 +10,14 @@
 //   * up to eight rows (one token of a model with up to eight query heads to a key head), P is a whole number of 16 bits, rn(65535 p) with p relative to the
 //     running maximum: its upper bytes make rows 0-7 of the product with V, its lower bytes rows 8-15.  Nothing is converted and no row is idle; the sums
 //     are exact and stay whole numbers until the maximum of a row grows.  2^-17 of the largest p for every key; fp16's 2^-12 of each p is no better where
-//     a row spreads over many keys, and 2900 instructions a tile became 800;
+//     a row spreads over many keys.  A batch of 64 sequences takes 1260 instructions a tile in all instead of 2870;
 //   * up to sixteen rows P is fp16 and V becomes fp16 in registers (integers up to 2048 are exact there), m16n8k16;
 //   * which key, column or row a lane's element belongs to is free as long as both operands agree, and is chosen so that each lane reads 16 bytes at a time
 //     without bank conflicts from the swizzled tiles, and so that the scores' registers are P's operand as they are;
 //   * the keys of a sequence are split over the warps of a cluster of CTAs, whose partial rows meet through distributed shared memory.
+//
+// 64 sequences of 1 to 8192 keys, 32 heads on 8 of 128: 106 to 109 us, 5.6 TB/s, 85 to 87 % of a copy's rate; 172 with P as fp16 (issue: 53 M instructions of six warps to an SM).
+// One sequence of 1025 keys: 7.9 us, latencies in a row.  Two of 125,000 keys on 4 key heads: 62 us on the 64 SMs that eight clusters of eight have, 4.1 TB/s.
 #pragma once
 #include "fmha_grouped_sm100.cuh"
 

@@ -198,21 +198,38 @@ template <int D, int kRows> int launch_rows(cudaStream_t stream, const Device& d
   const long long n_tiles = (c.max_k + grouped::kTile - 1) / grouped::kTile;
   if (units > kMostRows / rows::kMaxCluster) return FMHA_I8_ERR_TOO_LARGE;
   const long long resident = 3LL * dev.sm_count;
-  // Few units with many keys: one CTA with all the warps of an SM on as many SMs as a cluster allows.
+  // Few units with many keys: one CTA with all the warps of an SM on as many SMs as a cluster allows.  8 units of 131,072 keys, head_dim 128: 63 us; the CTAs of
+  // two warps below in clusters of 8 74, of 16 67 to 76.
   const int clusters16 = D == 128 ? g_once[dev.index].clusters16_d128 : g_once[dev.index].clusters16_d64;
   for (const int ctas : {16, 8})
     if (units * ctas <= dev.sm_count && (ctas == 8 || units <= clusters16) && n_tiles >= 2LL * ctas * Wide)
       return launch(rows::rows_kernel<D, Wide, kRows>, static_cast<unsigned>(units * ctas), Wide * 32, sizeof(rows::Smem<D, Wide, kRows>), stream, static_cast<unsigned>(ctas), mk, mv, p);
+  // Otherwise clusters as long as that fills the chip or takes a warp's tiles apart.  Against one CTA to a unit (us, head_dim 128): 8 units of 513 keys 8.0 and 10.3, of 8193
+  // 16 and 72; 128 of 1025 14.6 and 17.8; 512 of 4097 104 and 115; 256 of 300 10.4 and 10.3.
   int ctas = 1;
   while (ctas < 8 && ((units * ctas < 2 * resident && n_tiles >= 4 * ctas * W) || (units * ctas * 2 <= resident && n_tiles > ctas * W))) ctas *= 2;
   return launch(rows::rows_kernel<D, W, kRows>, static_cast<unsigned>(units * ctas), W * 32, sizeof(rows::Smem<D, W, kRows>), stream, static_cast<unsigned>(ctas), mk, mv, p);
 }
 
-// Up to 128 heads share a key head, and a tile of the chunk kernel holds at least one token.
-constexpr int kMostGroup = 128;
-bool few_rows(const grouped::Params& p) { return p.G > kMostGroup || static_cast<long long>(p.max_q) * p.G <= 16; }
+// Pairs of tiles of the chunk kernel: no more than the tokens make, and one more for every sequence.
+long long chunk_units(const grouped::Params& p) { return std::min<long long>(p.total_q, p.total_q / (2LL * (grouped::kTile / p.G)) + p.B) * p.Hkv; }
 
-// CTAs that share a unit of the chunk kernel, in steps of one key tile (1.8 us): a CTA's share of them, and 4 for what a part costs besides.
+// Which kernel.  Up to 128 heads share a key head of the chunk kernel, whose tile holds at least one token.  Otherwise by the rows of a sequence and key head
+// (rows kernel against chunk kernel, us): 16 rows, head_dim 128, 4097 keys: 8 units 15.6 and 17.8, 128 units 53 and 60, 512 units 119 and 223.
+// 17 to 32 rows are two groups of the rows kernel, each of which reads all keys: head_dim 64, 129 to 4097 keys, 8 to 1024 units: 0.47 to 0.87 of the chunk
+// kernel's time (512 units of 1025 keys 38 and 62); head_dim 128 0.78 to 0.93 of it for 512 units and more of 1025 keys and more (4097 keys 174 and 223),
+// 1.02 to 1.54 for fewer or shorter ones.  33 to 48 rows: 0.60 to 1.08 and 1.05 to 1.22.
+constexpr int kMostGroup = 128;
+bool few_rows(const Call& c, int sms) {
+  const grouped::Params& p = c.p;
+  const long long n_rows = static_cast<long long>(p.max_q) * p.G;
+  if (p.G > kMostGroup || n_rows <= 16) return true;
+  if (n_rows > 32) return false;
+  return c.D == 64 || (chunk_units(p) >= 3LL * sms && c.max_k > 7 * grouped::kTile);
+}
+
+// CTAs that share a unit of the chunk kernel, in steps of one key tile (1.7 us): a CTA's share of them, and 4 for what a part costs besides.  Without and with, us:
+// 200 tokens on 32,768 keys (B1 H32/8 D128) 469 and 138, two chunks of 103 on 88,000 (H24/12 D64) 1155 and 317, 16 on 4097 (B1 H32/8 D128) 57 and 20.
 int chunk_parts(long long units, long long n_tiles, int sms) {
   long long best = (units + sms - 1) / sms * (n_tiles + 2);
   int parts = 1;
@@ -234,8 +251,7 @@ template <int D> int launch_chunk(cudaStream_t stream, const Device& dev, Call& 
   if (!fn || fn(&mq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<int8_t*>(p.q), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
                 D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return FMHA_I8_ERR_DRIVER;
-  // pairs of tiles: no more than the tokens make, and one more for every sequence
-  const long long units = std::min<long long>(p.total_q, p.total_q / (2LL * p.tq) + p.B) * p.Hkv;
+  const long long units = chunk_units(p);
   if (units > kMostRows) return FMHA_I8_ERR_TOO_LARGE;
   const unsigned grid = static_cast<unsigned>(std::min<long long>(units, dev.sm_count));
   const int parts = chunk_parts(units, (c.max_k + grouped::kTile - 1) / grouped::kTile, dev.sm_count);
@@ -256,7 +272,7 @@ int run_attention(void* stream, Call& c) {
   if ((st = key_map(&mk, c.k, c.lk, c.D)) != FMHA_I8_OK) return st;
   if ((st = key_map(&mv, c.v, c.lv, c.D)) != FMHA_I8_OK) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (few_rows(c.p)) {
+  if (few_rows(c, dev.sm_count)) {
     if (static_cast<long long>(c.p.max_q) * c.p.G <= 8) return c.D == 128 ? launch_rows<128, 8>(s, dev, c, mk, mv) : launch_rows<64, 8>(s, dev, c, mk, mv);
     return c.D == 128 ? launch_rows<128, 16>(s, dev, c, mk, mv) : launch_rows<64, 16>(s, dev, c, mk, mv);
   }
@@ -370,7 +386,8 @@ int append_impl(void* stream, const float amax[5], const long long dims[5], cons
   if (st != FMHA_I8_OK || tokens == 0) return st;
   p.status = dev.status;
   p.host_word = dev.host_word;
-  // Warps that take one round of heads each, as long as that does not make more than the chip holds at once.
+  // Warps that take one round of heads each, up to 48 warps to an SM, then more rounds.  8192 tokens of 48 heads of 128: 42.9 us; with 96 warps 47.2, 160 53.4, 320 54.7 (a
+  // warp's later rounds have the table's entries and the position already, and the next heads on their way).
   const int at_once = static_cast<int>(512 / D), all = static_cast<int>((H + 2 * Hkv + at_once - 1) / at_once);
   const long long most_warps = 48LL * dev.sm_count;
   p.rounds = static_cast<int>(std::min<long long>(all, std::max<long long>(1, (tokens * all + most_warps - 1) / most_warps)));

@@ -387,6 +387,36 @@ def test_paged(pkg, torch, lens_q, lens_k, H, Hkv, D, page, out):
     run_paged(pkg, torch, lens_q, lens_k, H, Hkv, D, page, out, seed=H + D + page)
 
 
+# Up to 32 rows to a key head, on either side of what the kernels' choice looks at: rows (16, 17, 32, 33), key tiles (7, 8) and, for head_dim 128, the number of units.
+FEW_ROWS = [
+    # sequences, most tokens, most keys, H, Hkv, D, out
+    (3, 17, 300, 4, 4, 64, "bf16"),
+    (3, 8, 1500, 8, 2, 64, "fp16"),
+    (2, 11, 700, 6, 2, 64, "int8"),
+    (5, 1, 2100, 34, 2, 64, "bf16"),
+    (70, 8, 900, 32, 8, 128, "bf16"),
+    (70, 8, 897, 32, 8, 128, "int8"),
+    (70, 8, 896, 32, 8, 128, "bf16"),
+    (62, 17, 1100, 8, 8, 128, "fp16"),
+    (70, 11, 900, 24, 8, 128, "bf16"),
+    (40, 1, 1000, 320, 16, 128, "fp16"),
+]
+
+
+@pytest.mark.parametrize("sequences,tokens,keys,H,Hkv,D,out", FEW_ROWS)
+def test_paged_up_to_32_rows(pkg, torch, sequences, tokens, keys, H, Hkv, D, out):
+    lens_q = [tokens if b % 3 == 0 else (5 * b + 1) % (tokens + 1) for b in range(sequences)]
+    lens_k = [keys if b == 0 else n + (131 * b) % (keys + 1 - n) for b, n in enumerate(lens_q)]
+    run_paged(pkg, torch, lens_q, lens_k, H, Hkv, D, 32, out, seed=sequences + tokens)
+
+
+@pytest.mark.parametrize("D,sequences,keys", [(64, 4, 40), (128, 64, 930)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_packed_up_to_32_rows(pkg, torch, D, sequences, keys, causal):
+    lens_q = [(b * 7 + 8) % 9 for b in range(sequences)]
+    run_packed(pkg, torch, lens_q, [keys if b == 1 else (b * 97) % keys for b in range(sequences)], 24, 8, D, causal, "bf16", seed=D, max_q=9)
+
+
 def test_paged_other_forms(pkg, torch):
     run_paged(pkg, torch, [1, 50, 1], [333, 444, 5], 6, 3, 128, 16, "bf16", seed=1, together=True)
     run_paged(pkg, torch, [1, 50, 1], [333, 444, 5], 6, 3, 64, 32, "bf16", seed=2, causal=False)
