@@ -123,10 +123,13 @@ struct Failure {
 // ------------------------------------------------------------------------------------------------ units
 // The pairs of tiles of all sequences, the last of each sequence first, then the ones before those, and so on: with causal masks the ones with most keys
 // come first.  Every pair is one unit per key head.  CTA c takes units c, 2 grid - 1 - c, 2 grid + c, ...: a round in one direction, the next in the other.
+// The sequences are gone through in lots of 32, for the pairs of a level once, whatever number of units a CTA finds there: from the first one for every unit, 4096 prompts of 60 tokens (12 heads on
+// 4 of 64) took 1898 us instead of 468, 1024 of 100 328 instead of 208.
 template <int D, bool kSplit> __device__ __forceinline__ void walk_role(const Params& p, Ctl<D>* ctl) {
   const int lane = threadIdx.x & 31;
   const Failure fail{p, &ctl->abort};
   int level = -1, before = 0, here = 0;             // pairs of earlier levels, and of this one
+  int from = 0, passed = 0;                         // pairs of a CTA come in order: where the last one of this level was found, and how many lie before that
   bool checked = blockIdx.x != 0;
   auto pairs_of = [&](int b) {
     if (b >= p.B) return 0;
@@ -144,7 +147,7 @@ template <int D, bool kSplit> __device__ __forceinline__ void walk_role(const Pa
     while (more && (level < 0 || pair >= static_cast<long long>(before) + here)) {
       before += here;
       ++level;
-      here = 0;
+      here = from = passed = 0;
       if (p.B <= 32) here = __popc(__ballot_sync(0xFFFFFFFFu, few > level));
       else
         for (int b0 = 0; b0 < p.B; b0 += 32) here += __popc(__ballot_sync(0xFFFFFFFFu, pairs_of(b0 + lane) > level));
@@ -153,18 +156,18 @@ template <int D, bool kSplit> __device__ __forceinline__ void walk_role(const Pa
     }
     Unit unit{};
     if (more) {
-      int at = static_cast<int>(pair - before), b = 0, pairs = 0;
-      for (int b0 = 0;; b0 += 32) {
-        const int mine = p.B <= 32 ? few : pairs_of(b0 + lane);
+      int b = 0, pairs = 0;
+      for (int at = static_cast<int>(pair - before);; from += 32) {
+        const int mine = p.B <= 32 ? few : pairs_of(from + lane);
         const uint32_t with = __ballot_sync(0xFFFFFFFFu, mine > level);
         const int count = __popc(with);
-        if (at < count) {
-          const int src = __fns(with, 0u, at + 1);
-          b = b0 + src;
+        if (at < passed + count) {
+          const int src = __fns(with, 0u, at - passed + 1);
+          b = from + src;
           pairs = __shfl_sync(0xFFFFFFFFu, mine, src);
           break;
         }
-        at -= count;
+        passed += count;
       }
       unit.valid = 1;
       unit.b = b;
