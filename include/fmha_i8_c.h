@@ -162,8 +162,8 @@ int fmha_i8_sm100_infer_host_slice(const float amax[5], const int desc[4],
  * Serving a causal language model: rotary positions and the int8 cache, attention over packed prompts, attention over the cache.  The
  * reference has no counterpart.  Grouped heads: query heads h = 0 .. head_num - 1 read key head h / (head_num / head_num_kv).
  *
- * The scores are exact, the probabilities have 11 bits (fp16), or for up to eight query rows to a key head 16 bits of the largest, instead of the 8 of the calls above, and the sums 24: the output is that of the
- * softmax of the int8 inputs up to fp16 rounding of P, and the rounding to its own type.  Same bytes for the same call every time.
+ * The scores are exact, the probabilities have 11 bits (fp16) instead of the 8 of the calls above, or, up to eight query rows to a key head, 16
+ * bits of the row's largest, and the sums 24: the output is that of the softmax of the int8 inputs up to that rounding of P and the rounding to its own type.  Same bytes for the same call every time.
  *
  * desc6 = {batch_num, max_seq_q, max_seq_k, head_num, head_num_kv, head_dim}; head_dim 64 or 128, head_num a multiple of head_num_kv.
  * Lengths live on the device: cu_seqlens_q (int32 [batch_num + 1], ascending from the first token of the first sequence to the
@@ -171,6 +171,8 @@ int fmha_i8_sm100_infer_host_slice(const float amax[5], const int desc[4],
  * no key give zeros.  Tokens behind the last sequence are left as they were.  max_seq_q and max_seq_k are upper bounds of the lengths, by
  * which the work is divided; a longer sequence of keys is still computed in full, while tokens beyond max_seq_q may be left out (the device
  * status words say so: FMHA_I8_DEV_BAD_INDEX).  Offsets that point outside the tensors are cut to them and reported the same way.
+ * max_seq_k, or what the tensors can hold where that is less, goes up to 2^30, and with more than 16 query rows to a key head (max_seq_q * head_num / head_num_kv) up
+ * to 2^26: such a call with more may be refused with FMHA_I8_ERR_TOO_LARGE.
  * causal: token i of n_q sees keys j <= i + n_k - n_q, so that the last token sees all; without FMHA_I8_FLAG_CAUSAL all tokens see all keys.
  * q: int8, token t and head h at q + t * token stride + h * head_dim; o the same, int8 (requantised with amax[3] = o_amax), bf16 or fp16 (then
  * amax[3] is not looked at, nor is amax[4]).  All tensors 16-byte aligned, token strides in elements, whole multiples of 16 bytes.

@@ -220,6 +220,8 @@ long long chunk_units(const grouped::Params& p) { return std::min<long long>(p.t
 // kernel's time (512 units of 1025 keys 38 and 62); head_dim 128 0.78 to 0.93 of it for 512 units and more of 1025 keys and more (4097 keys 174 and 223),
 // 1.02 to 1.54 for fewer or shorter ones.  33 to 48 rows: 0.60 to 1.08 and 1.05 to 1.22.
 constexpr int kMostGroup = 128;
+// A warp of the chunk kernel may wait for a whole unit of another's, and gives up after about 1.5 s: 2^26 keys are 0.9 s.
+constexpr long long kMostChunkKeys = 1LL << 26;
 bool few_rows(const Call& c, int sms) {
   const grouped::Params& p = c.p;
   const long long n_rows = static_cast<long long>(p.max_q) * p.G;
@@ -268,11 +270,13 @@ int run_attention(void* stream, Call& c) {
   if (c.p.total_q == 0 || c.p.max_q == 0) return FMHA_I8_OK;
   c.p.status = dev.status;
   c.p.host_word = dev.host_word;
+  const bool few = few_rows(c, dev.sm_count);
+  if (!few && c.max_k > kMostChunkKeys) return FMHA_I8_ERR_TOO_LARGE;
   CUtensorMap mk, mv;
   if ((st = key_map(&mk, c.k, c.lk, c.D)) != FMHA_I8_OK) return st;
   if ((st = key_map(&mv, c.v, c.lv, c.D)) != FMHA_I8_OK) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (few_rows(c, dev.sm_count)) {
+  if (few) {
     if (static_cast<long long>(c.p.max_q) * c.p.G <= 8) return c.D == 128 ? launch_rows<128, 8>(s, dev, c, mk, mv) : launch_rows<64, 8>(s, dev, c, mk, mv);
     return c.D == 128 ? launch_rows<128, 16>(s, dev, c, mk, mv) : launch_rows<64, 16>(s, dev, c, mk, mv);
   }
@@ -291,6 +295,7 @@ int infer_packed_impl(void* stream, const float amax[5], const int desc6[6], con
   if (strides[1] % 16 != 0 || strides[2] % 16 != 0 || !aligned(cu_k, 4)) return FMHA_I8_ERR_MISALIGNED;
   c.p.cu_k = cu_k;
   c.p.total_k = static_cast<int>(tokens[1]);
+  c.max_k = std::min(c.max_k, tokens[1]);
   c.p.num_pages = 1;
   c.p.page_shift = 0;
   c.p.box_shift = log2_of(grouped::kTile);

@@ -225,6 +225,37 @@ def test_more_sequences_than_a_warp_has_lanes(pkg, torch):
     run_paged(pkg, torch, [1] * 150, [1 + (61 * i) % 500 for i in range(150)], 8, 2, 128, 16, "fp16", seed=4)
 
 
+@pytest.mark.parametrize("H,Hkv,D,causal", [(8, 1, 64, True), (4, 2, 128, False)])
+def test_hundreds_of_sequences_some_of_them_empty(pkg, torch, H, Hkv, D, causal):
+    """Units are found among the sequences in lots of 32: lots without a unit, one long sequence among short ones, ends inside a lot."""
+    lens = [0] * 70 + [(53 * i) % 90 for i in range(150)] + [700] + [0] * 40 + [1, 33, 200] + [20] * 60 + [0] * 33 + [129]
+    run_packed(pkg, torch, lens, None, H, Hkv, D, causal, "bf16", seed=D)
+
+
+def test_more_keys_than_waits_are_sized_for(pkg, torch):
+    """Chunks on more than 2^26 keys are refused, single tokens are not; a bound that the tensors do not reach does not count."""
+    kc = torch.zeros((1, 1, 4096, 64), dtype=torch.int8, device="cuda")
+    q = torch.zeros((40, 1, 64), dtype=torch.int8, device="cuda")
+    o = torch.empty((40, 1, 64), dtype=torch.bfloat16, device="cuda")
+    lens = torch.tensor([50], dtype=torch.int32, device="cuda")
+    for width, tokens, most, refused in ((1 << 15, 40, 1 << 27, True), (1 << 15, 40, (1 << 26) + 1, True), (1 << 15, 40, 1 << 26, False), (1 << 15, 4, 1 << 27, False),
+                                         (1 << 14, 40, 1 << 27, False)):
+        table = torch.zeros((1, width), dtype=torch.int32, device="cuda")
+        args = (None, param(pkg), pkg.AttnDataDescriptorGrouped(1, tokens, most, 1, 1, 64), q[:tokens], kc, kc, table, lens, starts([tokens]), o[:tokens])
+        if refused:
+            with pytest.raises(pkg.FmhaError) as e:
+                pkg.FMHAInferI8Paged(*args)
+            assert e.value.status == pkg.ERR_TOO_LARGE
+        else:
+            o.fill_(7.0)
+            pkg.FMHAInferI8Paged(*args)
+            assert bool((o[:tokens] == 0).all())
+    k = torch.zeros((50, 1, 64), dtype=torch.int8, device="cuda")
+    o.fill_(7.0)
+    pkg.FMHAInferI8Packed(None, param(pkg), pkg.AttnDataDescriptorGrouped(1, 40, 1 << 30, 1, 1, 64), q, k, k, starts([40]), starts([50]), o)
+    assert bool((o == 0).all())
+
+
 @pytest.mark.parametrize("out", ["bf16", "int8"])
 def test_outputs_with_strides_and_the_least_alignment(pkg, torch, out):
     """o as a view with a row of its own spacing, 16-byte aligned only: the narrow stores, and nothing besides the rows is touched."""
