@@ -135,12 +135,12 @@ template <int D, bool kSplit> __device__ __forceinline__ void walk_role(const Pa
     if (b >= p.B) return 0;
     const Seq s = load_seq(p, b);
     if (!checked && (s.bad)) report(p.status, p.host_word, FMHA_I8_DEV_BAD_INDEX, 0u, b);
-    return (s.nq + 2 * p.tq - 1) / (2 * p.tq);
+    return s.nq * p.G <= p.few_rows ? 0 : (s.nq + 2 * p.tq - 1) / (2 * p.tq);
   };
   const int few = p.B <= 32 ? pairs_of(lane) : 0;   // up to 32 sequences: kept in registers
   for (uint32_t n = 0;; ++n) {
     const long long round = n, ctas = gridDim.x;
-    const long long u = kSplit ? static_cast<long long>(blockIdx.x / cluster_ctas()) : round * ctas + ((n & 1u) ? ctas - 1 - blockIdx.x : blockIdx.x);
+    const long long u = kSplit ? static_cast<long long>(blockIdx.x / cluster_ctas()) : p.first_unit + round * ctas + ((n & 1u) ? ctas - 1 - blockIdx.x : blockIdx.x);
     const int head = static_cast<int>(u % p.Hkv);
     const long long pair = u / p.Hkv;
     bool more = !kSplit || n == 0;

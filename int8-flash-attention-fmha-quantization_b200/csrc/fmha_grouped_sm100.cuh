@@ -41,6 +41,8 @@ struct Params {
   int o_wide;                          // rows of o are 32-byte aligned
   int row_groups;                      // rows kernel: groups of 16 rows per sequence and key head
   int tq;                              // chunk kernel: tokens per tile of 128 rows
+  int few_rows;                        // 0, or: sequences with up to this many rows to a key head are the rows kernel's, the others the chunk kernel's
+  long long first_unit;                // chunk kernel, units not split: those before this one are another launch's
   float c2;                            // from a difference of scores to an exponent of 2
   int growth;                          // chunk kernel: a reference is kept while the maximum exceeds it by no more than this, 2^14 in p
   float out_scale;                     // from sum p v / sum p, v in codes, to the output's unit

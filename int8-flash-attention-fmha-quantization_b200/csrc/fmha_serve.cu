@@ -193,7 +193,7 @@ int fill_call(Call* c, const float amax[5], const int desc6[6], const void* q, c
 template <int D, int kRows> int launch_rows(cudaStream_t stream, const Device& dev, Call& c, const CUtensorMap& mk, const CUtensorMap& mv) {
   grouped::Params& p = c.p;
   constexpr int W = RowsCfg<D>::kWarps, Wide = RowsCfg<D>::kWarpsWide;
-  p.row_groups = static_cast<int>((static_cast<long long>(p.max_q) * p.G + kRows - 1) / kRows);
+  p.row_groups = p.few_rows != 0 ? 1 : static_cast<int>((static_cast<long long>(p.max_q) * p.G + kRows - 1) / kRows);
   const long long units = static_cast<long long>(p.B) * p.Hkv * p.row_groups;
   const long long n_tiles = (c.max_k + grouped::kTile - 1) / grouped::kTile;
   if (units > kMostRows / rows::kMaxCluster) return FMHA_I8_ERR_TOO_LARGE;
@@ -232,14 +232,31 @@ bool few_rows(const Call& c, int sms) {
 
 // CTAs that share a unit of the chunk kernel, in steps of one key tile (1.7 us): a CTA's share of them, and 4 for what a part costs besides.  Without and with, us:
 // 200 tokens on 32,768 keys (B1 H32/8 D128) 469 and 138, two chunks of 103 on 88,000 (H24/12 D64) 1155 and 317, 16 on 4097 (B1 H32/8 D128) 57 and 20.
-int chunk_parts(long long units, long long n_tiles, int sms) {
-  long long best = (units + sms - 1) / sms * (n_tiles + 2);
-  int parts = 1;
+struct Split { int parts; long long steps; };
+Split chunk_split(long long units, long long n_tiles, int sms) {
+  Split best{1, (units + sms - 1) / sms * (n_tiles + 2)};
   for (const int c : {2, 4, 8}) {
-    const long long rounds = (units * c + sms - 1) / sms, cost = rounds * ((n_tiles + c - 1) / c + 4);
-    if (cost < best) { best = cost; parts = c; }
+    const long long rounds = (units * c + sms - 1) / sms, steps = rounds * ((n_tiles + c - 1) / c + 4);
+    if (steps < best.steps) best = Split{c, steps};
   }
-  return parts;
+  return best;
+}
+// In a mixed batch, where most sequences bring a token or two: the units that there are if the others have as many tokens as they may.
+long long expected_units(const grouped::Params& p) {
+  return std::min(chunk_units(p), (p.total_q / (2LL * (grouped::kTile / p.G)) + (p.total_q + p.max_q - 1) / p.max_q) * p.Hkv);
+}
+// The rows of sequences that the rows kernel takes out of a batch of chunks, or 0.  The host does not know the lengths, but the tokens that there are in all: below a quarter of
+// what the sequences may bring.  Steps of the chunk kernel with all sequences against those with the expected ones, 8 for two more launches and the rows kernel's tiles, of
+// which 300 take a step.  In one launch and apart, us (H32/8 D128 where not said): one chunk of 512 among 64 sequences of up to 4096 keys 177 and 118, two of 1024 among 256 of up
+// to 8192 1016 and 596, two of 2048 among 130 288 and 202, one of 480 among 33 of up to 4096 (H16/2 D64) 60 and 52; left in one launch: one of 500 among 5 of up to 1000 20 and 39, 15 of
+// 256 among 64 (H12/1) 56 and 71, 8 of 300 among 33 85 and 83.
+int rows_apart(const Call& c, int sms) {
+  const grouped::Params& p = c.p;
+  if (p.G > 16 || 4LL * p.total_q > static_cast<long long>(p.B) * p.max_q) return 0;
+  const long long n_tiles = (c.max_k + grouped::kTile - 1) / grouped::kTile;
+  const long long apart = chunk_split(expected_units(p), n_tiles, sms).steps + 8 + static_cast<long long>(p.B) * p.Hkv * n_tiles / 300;
+  if (apart >= chunk_split(chunk_units(p), n_tiles, sms).steps) return 0;
+  return p.G <= 8 ? 8 : 16;
 }
 
 template <int D> int launch_chunk(cudaStream_t stream, const Device& dev, Call& c, const CUtensorMap& mk, const CUtensorMap& mv) {
@@ -255,10 +272,15 @@ template <int D> int launch_chunk(cudaStream_t stream, const Device& dev, Call& 
     return FMHA_I8_ERR_DRIVER;
   const long long units = chunk_units(p);
   if (units > kMostRows) return FMHA_I8_ERR_TOO_LARGE;
-  const unsigned grid = static_cast<unsigned>(std::min<long long>(units, dev.sm_count));
-  const int parts = chunk_parts(units, (c.max_k + grouped::kTile - 1) / grouped::kTile, dev.sm_count);
-  if (parts > 1)
-    return launch(chunk::chunk_kernel<D, true, true>, static_cast<unsigned>(units * parts), chunk::kThreads, chunk::smem_bytes<D>(), stream, static_cast<unsigned>(parts), mq, mk, mv, p);
+  // In a mixed batch the expected units may be shared by clusters; what goes beyond them is left to a second launch, which mostly finds nothing.
+  const long long expected = p.few_rows == 0 ? units : expected_units(p);
+  const int parts = chunk_split(expected, (c.max_k + grouped::kTile - 1) / grouped::kTile, dev.sm_count).parts;
+  if (parts > 1) {
+    const int st = launch(chunk::chunk_kernel<D, true, true>, static_cast<unsigned>(expected * parts), chunk::kThreads, chunk::smem_bytes<D>(), stream, static_cast<unsigned>(parts), mq, mk, mv, p);
+    if (st != FMHA_I8_OK || expected == units) return st;
+    p.first_unit = expected;
+  }
+  const unsigned grid = static_cast<unsigned>(std::min<long long>(units - p.first_unit, dev.sm_count));
   return launch(p.c2 > 0.5f ? chunk::chunk_kernel<D, true, false> : chunk::chunk_kernel<D, false, false>, grid, chunk::kThreads, chunk::smem_bytes<D>(), stream, 0u, mq, mk, mv, p);
 }
 
@@ -276,9 +298,12 @@ int run_attention(void* stream, Call& c) {
   if ((st = key_map(&mk, c.k, c.lk, c.D)) != FMHA_I8_OK) return st;
   if ((st = key_map(&mv, c.v, c.lv, c.D)) != FMHA_I8_OK) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (few) {
-    if (static_cast<long long>(c.p.max_q) * c.p.G <= 8) return c.D == 128 ? launch_rows<128, 8>(s, dev, c, mk, mv) : launch_rows<64, 8>(s, dev, c, mk, mv);
-    return c.D == 128 ? launch_rows<128, 16>(s, dev, c, mk, mv) : launch_rows<64, 16>(s, dev, c, mk, mv);
+  if (!few) c.p.few_rows = rows_apart(c, dev.sm_count);
+  if (few || c.p.few_rows != 0) {
+    const bool eight = few ? static_cast<long long>(c.p.max_q) * c.p.G <= 8 : c.p.few_rows == 8;
+    if (c.D == 128) st = eight ? launch_rows<128, 8>(s, dev, c, mk, mv) : launch_rows<128, 16>(s, dev, c, mk, mv);
+    else st = eight ? launch_rows<64, 8>(s, dev, c, mk, mv) : launch_rows<64, 16>(s, dev, c, mk, mv);
+    if (few || st != FMHA_I8_OK) return st;
   }
   return c.D == 128 ? launch_chunk<128>(s, dev, c, mk, mv) : launch_chunk<64>(s, dev, c, mk, mv);
 }

@@ -45,8 +45,9 @@ def attention64(q, k, v, amax, causal):
     return (p @ vv).transpose(0, 1) * real, ((p @ vv.abs()).transpose(0, 1) * real, each.transpose(0, 1) * real)
 
 
-def tolerance(o, scales, keys, o_type, amax, o_amax, rows):
-    """Elementwise bound of |result - o|, o in real units.  `rows`: query rows per key head that the call allows (max_seq_q * heads of a group).
+def tolerance(o, scales, keys, o_type, amax, o_amax, rows, own=None):
+    """Elementwise bound of |result - o|, o in real units.  `rows`: query rows per key head that the call allows (max_seq_q * heads of a group); `own`: those that the
+    sequence has.  In a call that allows more than eight, a sequence with up to eight may be computed with either P (below), so the larger bound holds.
       P        fp16: half a step, 2^-11 relative, of every p; below 2^-14 half a step is 2^-25 of the row's largest p, which is 1 or more.  Up to eight rows: whole
                numbers of 16 bits, half a step, 2^-17 of the largest p, for every key.
       exp2     2^-22; its argument (|a| <= 24 where p matters) is off by half a step of the factor and of its rounding (2^-24 relative each) and, up to
@@ -56,7 +57,8 @@ def tolerance(o, scales, keys, o_type, amax, o_amax, rows):
     out = torch.full_like(o, 0.5 * o_amax / 127.0) if o_type == "int8" else o.abs() * (torch.finfo(TYPES[o_type]).eps / 2)
     tiny = 0.0 if o_type != "fp16" else 2.0 ** -25            # half a step below fp16's smallest normal number
     spread, each = scales
-    of_p = each * 2.0 ** -17 if rows <= 8 else spread * 2.0 ** -11 + each * 2.0 ** -25
+    whole, half = each * 2.0 ** -17, spread * 2.0 ** -11 + each * 2.0 ** -25
+    of_p = whole if rows <= 8 else half if own is None or own > 8 else torch.maximum(whole, half)
     return out * 1.001 + of_p + spread * (2.0 ** -18 + keys * 2.0 ** -24) + tiny + 1e-12
 
 
@@ -64,10 +66,10 @@ def real_units(o, o_type, o_amax):
     return o.double() * (o_amax / 127.0) if o_type == "int8" else o.double()
 
 
-def check(got, want, scales, keys, o_type, amax, o_amax, rows, what=""):
+def check(got, want, scales, keys, o_type, amax, o_amax, rows, what="", own=None):
     want_c = want.clamp(-o_amax, o_amax) if o_type == "int8" else want
     err = (real_units(got, o_type, o_amax) - want_c).abs()
-    tol = tolerance(want_c, scales, keys, o_type, amax, o_amax, rows)
+    tol = tolerance(want_c, scales, keys, o_type, amax, o_amax, rows, own)
     over = err > tol
     assert not bool(over.any()), f"{what}: {int(over.sum())} of {over.numel()} off, worst {float((err / tol).max()):.3g} times the tolerance"
 

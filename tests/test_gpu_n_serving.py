@@ -171,7 +171,7 @@ def run_packed(pkg, torch, lens_q, lens_k, H, Hkv, D, causal, out, seed, tail=3,
     at_q = at_k = 0
     for n, m in zip(lens_q, lens_k):
         want, spread = attention64(q[at_q:at_q + n], k[at_k:at_k + m], v[at_k:at_k + m], AMAX, causal)
-        check(o[at_q:at_q + n], want, spread, m, out, AMAX, O_AMAX, desc.max_seq_q * H // Hkv, f"{n} tokens on {m} keys")
+        check(o[at_q:at_q + n], want, spread, m, out, AMAX, O_AMAX, desc.max_seq_q * H // Hkv, f"{n} tokens on {m} keys", own=n * H // Hkv)
         at_q += n
         at_k += m
     assert bool((o[at_q:] == FILL[out]).all()), "tokens behind the last sequence were touched"
@@ -230,6 +230,96 @@ def test_hundreds_of_sequences_some_of_them_empty(pkg, torch, H, Hkv, D, causal)
     """Units are found among the sequences in lots of 32: lots without a unit, one long sequence among short ones, ends inside a lot."""
     lens = [0] * 70 + [(53 * i) % 90 for i in range(150)] + [700] + [0] * 40 + [1, 33, 200] + [20] * 60 + [0] * 33 + [129]
     run_packed(pkg, torch, lens, None, H, Hkv, D, causal, "bf16", seed=D)
+
+
+def run_mixed(pkg, torch, lens_q, lens_k, max_q, H, Hkv, D, out, seed, causal=True):
+    """As run_paged, with a bound of the tokens that need not be reached; how many launches it took."""
+    kc, vc, table, lens = make_cache(torch, lens_k, Hkv, D, 32, seed)
+    T = sum(lens_q) + 2
+    q = codes((T, H, D), seed + 5)
+    o = torch.full((T, H, D), FILL[out], dtype=TYPES[out], device="cuda")
+    before = pkg.launch_count()
+    pkg.FMHAInferI8Paged(None, param(pkg), pkg.AttnDataDescriptorGrouped(len(lens_q), max_q, max(lens_k), H, Hkv, D), q, kc, vc, table, lens, starts(lens_q), o, causal=causal)
+    launches = pkg.launch_count() - before
+    at = 0
+    for b, (n, m) in enumerate(zip(lens_q, lens_k)):
+        want, spread = attention64(q[at:at + n], keys_of(kc, table, b, m), keys_of(vc, table, b, m), AMAX, causal)
+        check(o[at:at + n], want, spread, m, out, AMAX, O_AMAX, max_q * H // Hkv, f"sequence {b}: {n} tokens on {m} keys", own=n * H // Hkv)
+        at += n
+    assert bool((o[at:] == FILL[out]).all())
+    return launches
+
+
+# (the launches that a B200 with 148 SMs makes: one, or the single tokens' and the chunks', or a third for more units than were expected)
+MIXED = [
+    # tokens of the sequences that bring many, (bound), sequences with few, most keys, H, Hkv, D, out
+    ([480], 480, 32, 3000, 16, 2, 64, "bf16"),
+    ([300, 17, 120], 300, 61, 2100, 32, 8, 128, "bf16"),
+    ([300, 200], 300, 70, 1500, 8, 2, 128, "int8"),
+    ([200] * 3, 1000, 30, 8000, 24, 2, 64, "fp16"),
+    ([3] * 60, 700, 2, 3000, 32, 8, 128, "bf16"),          # not one that brings many: three tokens each are twelve rows
+    ([40] * 90, 900, 0, 2500, 16, 4, 64, "bf16"),          # a bound that nobody reaches: many more units than were expected
+    ([], 2000, 64, 4000, 32, 8, 128, "fp16"),              # nothing but single tokens
+]
+
+
+@pytest.mark.parametrize("many,max_q,few,keys,H,Hkv,D,out", MIXED)
+def test_paged_single_tokens_among_chunks(pkg, torch, many, max_q, few, keys, H, Hkv, D, out):
+    most = max(1, (8 if H // Hkv <= 8 else 16) * Hkv // H)              # tokens that the kernel for few rows takes
+    lens_q = [1 + i % most if i % 11 else 0 for i in range(few)]
+    for i, n in enumerate(many):
+        lens_q.insert((7 * i) % (len(lens_q) + 1), n)
+    lens_k = [keys if b == len(lens_q) // 2 else n + (277 * b) % (keys - n) for b, n in enumerate(lens_q)]
+    assert run_mixed(pkg, torch, lens_q, lens_k, max_q, H, Hkv, D, out, seed=H + keys) > 1
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_paged_a_token_more_than_the_kernel_for_few_rows_takes(pkg, torch, causal):
+    for G, tokens in ((2, (4, 5)), (3, (2, 3)), (8, (1, 2)), (16, (1, 2)), (1, (8, 9))):
+        lens_q = [tokens[i % 2] for i in range(60)] + [400]
+        run_mixed(pkg, torch, lens_q, [900 + 31 * i for i in range(61)], 400, 4 * G, 4, 64, "bf16", seed=G, causal=causal)
+
+
+# On 148 SMs 65 sequences stay in one launch -- 22 steps apart, 8 of them the launches, against 22 -- while 193 do not: 12 + 8 + 66 against 168.
+@pytest.mark.parametrize("lots,apart", [(16, False), (48, True)])
+def test_packed_single_tokens_among_chunks(pkg, torch, lots, apart):
+    lens_q, lens_k, H, Hkv, D = [1, 2, 0, 1] * lots + [350], [40 + 17 * i for i in range(4 * lots)] + [1100], 16, 4, 128
+    q, k, v = codes((sum(lens_q), H, D), 1), codes((sum(lens_k), Hkv, D), 2), codes((sum(lens_k), Hkv, D), 3)
+    o = torch.full((sum(lens_q), H, D), 77.0, dtype=torch.bfloat16, device="cuda")
+    before = pkg.launch_count()
+    pkg.FMHAInferI8Packed(None, param(pkg), pkg.AttnDataDescriptorGrouped(4 * lots + 1, 350, max(lens_k), H, Hkv, D), q, k, v, starts(lens_q), starts(lens_k), o)
+    assert (pkg.launch_count() - before > 1) == apart
+    i = j = 0
+    for n, m in zip(lens_q, lens_k):
+        want, spread = attention64(q[i:i + n], k[j:j + m], v[j:j + m], AMAX, True)
+        check(o[i:i + n], want, spread, m, "bf16", AMAX, O_AMAX, 350 * H // Hkv, f"{n} tokens on {m} keys", own=n * H // Hkv)
+        i, j = i + n, j + m
+
+
+def test_a_captured_mixed_step_follows_its_lengths(pkg, torch):
+    """The same call with other lengths on the device: chunks where single tokens were, and the other way round."""
+    B, H, Hkv, D, T, max_q = 40, 16, 4, 128, 700, 400
+    lens_k = [2500 - 13 * b for b in range(B)]
+    kc, vc, table, lens = make_cache(torch, lens_k, Hkv, D, 64, 3)
+    q = codes((T, H, D), 8)
+    o = torch.zeros((T, H, D), dtype=torch.bfloat16, device="cuda")
+    cu = torch.zeros(B + 1, dtype=torch.int32, device="cuda")
+    args = (param(pkg), pkg.AttnDataDescriptorGrouped(B, max_q, 2500, H, Hkv, D), q, kc, vc, table, lens, cu, o)
+    pkg.FMHAInferI8Paged(None, *args)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        pkg.FMHAInferI8Paged(torch.cuda.current_stream().cuda_stream, *args)
+    for lens_q in ([1] * 39 + [400], [400] + [2] * 10 + [1] * 29, [17] * 40, [0] * 20 + [1] * 20, [200, 3, 200] + [1] * 37):
+        cu.copy_(starts(lens_q))
+        o.fill_(77.0)
+        graph.replay()
+        at = 0
+        for b, n in enumerate(lens_q):
+            want, spread = attention64(q[at:at + n], keys_of(kc, table, b, lens_k[b]), keys_of(vc, table, b, lens_k[b]), AMAX, True)
+            check(o[at:at + n], want, spread, lens_k[b], "bf16", AMAX, O_AMAX, max_q * H // Hkv, f"{n} tokens", own=n * H // Hkv)
+            at += n
+        assert bool((o[at:] == 77.0).all())
 
 
 def test_more_keys_than_waits_are_sized_for(pkg, torch):
@@ -384,7 +474,7 @@ def run_paged(pkg, torch, lens_q, lens_k, H, Hkv, D, page, out, seed, causal=Tru
     at = 0
     for b, (n, m) in enumerate(zip(lens_q, lens_k)):
         want, spread = attention64(q[at:at + n], keys_of(kc, table, b, m), keys_of(vc, table, b, m), AMAX, causal)
-        check(o[at:at + n], want, spread, m, out, AMAX, O_AMAX, desc.max_seq_q * H // Hkv, f"sequence {b}: {n} tokens on {m} keys")
+        check(o[at:at + n], want, spread, m, out, AMAX, O_AMAX, desc.max_seq_q * H // Hkv, f"sequence {b}: {n} tokens on {m} keys", own=n * H // Hkv)
         at += n
     assert bool((o[at:] == FILL[out]).all())
 
