@@ -280,6 +280,11 @@ def test_paged_a_token_more_than_the_kernel_for_few_rows_takes(pkg, torch, causa
         run_mixed(pkg, torch, lens_q, [900 + 31 * i for i in range(61)], 400, 4 * G, 4, 64, "bf16", seed=G, causal=causal)
 
 
+def test_a_chunk_longer_than_its_bound_in_a_mixed_batch(pkg, torch):
+    """It is computed in full, as in a batch of chunks alone, and nothing is reported (the fixture looks)."""
+    assert run_mixed(pkg, torch, [1] * 20 + [480] + [1] * 20, [2000 + 50 * b for b in range(41)], 400, 16, 2, 64, "bf16", seed=12) > 1
+
+
 # On 148 SMs 65 sequences stay in one launch -- 22 steps apart, 8 of them the launches, against 22 -- while 193 do not: 12 + 8 + 66 against 168.
 @pytest.mark.parametrize("lots,apart", [(16, False), (48, True)])
 def test_packed_single_tokens_among_chunks(pkg, torch, lots, apart):
