@@ -163,8 +163,8 @@ int fmha_i8_sm100_infer_host_slice(const float amax[5], const int desc[4],
  * reference has no counterpart.  Grouped heads: query heads h = 0 .. head_num - 1 read key head h / (head_num / head_num_kv).
  *
  * The scores are exact, the probabilities have 11 bits (fp16) instead of the 8 of the calls above, or, for a sequence of up
- * to eight query rows (tokens * head_num / head_num_kv), 16 bits of the row's largest, and the sums 24: the output is that of the softmax of the
- * int8 inputs up to that rounding of P and the rounding to its own type.  Same bytes for the same call every time.
+ * to eight query rows (tokens * head_num / head_num_kv), are whole numbers of 16 or 32 bits that are as good, and the sums have 24: the output is that of the
+ * softmax of the int8 inputs up to that rounding of P and the rounding to its own type.  Same bytes for the same call every time.
  *
  * desc6 = {batch_num, max_seq_q, max_seq_k, head_num, head_num_kv, head_dim}; head_dim 64 or 128, head_num a multiple of head_num_kv.
  * Lengths live on the device: cu_seqlens_q (int32 [batch_num + 1], ascending from the first token of the first sequence to the

@@ -4,9 +4,9 @@
 // For every token i of a sequence with n_q query tokens and n_k keys, and every head h with key head h / G:
 //   o_i = sum_j softmax_j(c q_i . k_j) v_j,   c = q_amax k_amax / (127^2 sqrt(D)),   j < n_k and, causal, j <= i + n_k - n_q
 // (the last query token sees all keys).  A token that sees no key gives zeros.  The scores are exact integers, the probabilities
-// p = 2^(c log2(e) (s - m)) are rounded to fp16 for P.V (11 bits: half a step is 2^-12 of a p that is not subnormal), whose other operand, the int8 values, fp16 holds
-// exactly; up to eight rows, to whole numbers rn(65535 p), 2^-17 of the row's largest.  Products are summed in fp32 (those of whole numbers exactly, in 32 bits, before that), and so is
-// the row sum, of the unrounded p.  (8 bits for P, as in the padded calls of this library,
+// p = 2^(c log2(e) (s - m)) are rounded to fp16 for P.V (11 bits: half a step is 2^-11 of a p that is not subnormal, at most), whose other operand, the int8 values, fp16
+// holds exactly; up to eight rows, to whole numbers of 32 bits, or of 16 where these add up to errors of 2^-11 of a tile's weight at most (fmha_rows_sm100.cuh).  Products
+// are summed in fp32 (those of whole numbers exactly, in 32 bits, before that), and so is the row sum, of the unrounded p.  (8 bits for P, as in the padded calls of this library,
 // would be 2^-8 of the largest p for every key: 3 % of the output of a row that spreads over 4096 keys.)
 #pragma once
 #include <cuda.h>

@@ -117,8 +117,8 @@ int set_up(const Device& dev) {
   std::lock_guard<std::mutex> lock(g_once_mutex);
   if (once.done.load(std::memory_order_relaxed)) return FMHA_I8_OK;
   int st;
-  if ((st = set_up_rows<64, 8>()) != FMHA_I8_OK || (st = set_up_rows<64, 16>()) != FMHA_I8_OK) return st;
-  if ((st = set_up_rows<128, 8>()) != FMHA_I8_OK || (st = set_up_rows<128, 16>()) != FMHA_I8_OK) return st;
+  if ((st = set_up_rows<64, 4>()) != FMHA_I8_OK || (st = set_up_rows<64, 8>()) != FMHA_I8_OK || (st = set_up_rows<64, 16>()) != FMHA_I8_OK) return st;
+  if ((st = set_up_rows<128, 4>()) != FMHA_I8_OK || (st = set_up_rows<128, 8>()) != FMHA_I8_OK || (st = set_up_rows<128, 16>()) != FMHA_I8_OK) return st;
   once.clusters16_d64 = count_clusters<64>();
   once.clusters16_d128 = count_clusters<128>();
   if ((st = set_up_chunk<64>()) != FMHA_I8_OK || (st = set_up_chunk<128>()) != FMHA_I8_OK) return st;
@@ -300,9 +300,9 @@ int run_attention(void* stream, Call& c) {
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (!few) c.p.few_rows = rows_apart(c, dev.sm_count);
   if (few || c.p.few_rows != 0) {
-    const bool eight = few ? static_cast<long long>(c.p.max_q) * c.p.G <= 8 : c.p.few_rows == 8;
-    if (c.D == 128) st = eight ? launch_rows<128, 8>(s, dev, c, mk, mv) : launch_rows<128, 16>(s, dev, c, mk, mv);
-    else st = eight ? launch_rows<64, 8>(s, dev, c, mk, mv) : launch_rows<64, 16>(s, dev, c, mk, mv);
+    const long long rows = few ? static_cast<long long>(c.p.max_q) * c.p.G : c.p.few_rows;
+    if (c.D == 128) st = rows <= 4 ? launch_rows<128, 4>(s, dev, c, mk, mv) : rows <= 8 ? launch_rows<128, 8>(s, dev, c, mk, mv) : launch_rows<128, 16>(s, dev, c, mk, mv);
+    else st = rows <= 4 ? launch_rows<64, 4>(s, dev, c, mk, mv) : rows <= 8 ? launch_rows<64, 8>(s, dev, c, mk, mv) : launch_rows<64, 16>(s, dev, c, mk, mv);
     if (few || st != FMHA_I8_OK) return st;
   }
   return c.D == 128 ? launch_chunk<128>(s, dev, c, mk, mv) : launch_chunk<64>(s, dev, c, mk, mv);
