@@ -12,15 +12,15 @@
 //   warp 14          turns unit numbers into sequences, tiles and key ranges, ahead of the others
 //
 // The output stays in tensor memory for a whole unit: a row's exponentials are taken relative to a reference that follows the running
-// maximum only when that has grown by more than 2^14 in p, which fp16 holds, and then the output is rescaled in place.  That is rare
-// behind a row's first keys.
+// maximum only when that has grown by more than 2^8 in p, and then the output is rescaled in place.  That is rare behind a row's first keys.  P is 2^7 at the
+// reference: fp16 holds 2^15, and its smallest step, 2^-24, is 2^-31 of that, so that many keys far below one are not lost.
 // Tensor memory (512 columns): S of A, of B (128 columns each; P as fp16 over the first 64), O of A, of B (128 each).
 //
 // What bounds it: a tile's chain scores - softmax - P.V - scores.  A step of both tiles takes 3300 cycles: 220 from the scores' barrier to registers, 350 for the maximum, 1900 for 128
 // exponentials and their conversion (in halves, P.V of the first beside the second), 770 for P.V and the next scores.  The tiles run half a step apart, so that one's
 // exponentials hide the other's products; a third would need tensor memory that there is not.  A unit's end takes 3700 cycles: the output is read, scaled and stored while the tensor
 // cores have only the other tile.  Tensor pipe 45 % of the cycles, issue 45 %, HBM 9 %.
-//   1 x 16384 tokens, 32 heads on 8 of 128, causal, some values eight times as large   1720 us, 1.28 PFLOP/s (1.34 without those values: references that move)
+//   1 x 16384 tokens, 32 heads on 8 of 128, causal, some values eight times as large   1765 us, 1.25 PFLOP/s (1.35 without those values: references that move)
 //   8 x 2048 tokens                                                                     247 us, 1.11 PFLOP/s; among other calls, at the power limit, 1800 and 267
 #pragma once
 #include "fmha_grouped_sm100.cuh"
@@ -40,6 +40,7 @@ constexpr int kInfoConsumers = 8 + 4 + 1 + 2;      // softmax warps, converters,
 constexpr uint32_t kTmemCols = 512;
 // Scores come as the bits of the float kMagic + score (see issue_scores), which order like integers.
 constexpr int kLowest = static_cast<int>(kMagicBits) - (1 << 22);        // below every score (127 * 127 * 128 < 2^21)
+constexpr float kLift = 7.f;                                             // P is 2^kLift at the reference, and 2^kGrowth more at most
 constexpr uint32_t kMasked = 0xFF000000u;                                // -2^127: below that, and its exponential is zero
 
 template <int D> struct Cfg {
@@ -456,7 +457,7 @@ template <int D, bool kWide, bool kSplit> __device__ __forceinline__ void softma
     const bool any = __any_sync(0xFFFFFFFFu, limit > 0);            // a warp without a row that sees a key leaves its part of P as it is
     const int least = __reduce_min_sync(0xFFFFFFFFu, real ? limit : 0x7FFFFFFF);      // keys that all rows see
     // p = 2^((x - ref) c2), x and ref as the floats kMagic + score.  Exponents are x c2 - hi with hi = ref c2 rounded, the same for a row as long as its
-    // reference is, and rounded once.  Where c2 is large the difference is taken first: hi would be off by as much as 16.
+    // reference is, and rounded once.  (kLift is in hi.)  Where c2 is large the difference is taken first: hi would be off by as much as 16.
     int ref = 0;
     float hi = 0.f;
     float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
@@ -492,12 +493,12 @@ template <int D, bool kWide, bool kSplit> __device__ __forceinline__ void softma
         const int m = max(m0, m1);
         if (i == 0) {
           ref = m;
-          hi = __int_as_float(m) * p.c2;
+          hi = fmaf(__int_as_float(m), p.c2, -kLift);
         } else {
           const bool grown = m - ref > p.growth;
           if (__any_sync(0xFFFFFFFFu, grown)) {
             grew = true;
-            const float next = grown ? __int_as_float(m) * p.c2 : hi;
+            const float next = grown ? fmaf(__int_as_float(m), p.c2, -kLift) : hi;
             factor = !grown ? 1.f : kWide ? ex2((__int_as_float(ref) - __int_as_float(m)) * p.c2) : ex2(hi - next);
             if (grown) ref = m;
             hi = next;
@@ -529,7 +530,7 @@ template <int D, bool kWide, bool kSplit> __device__ __forceinline__ void softma
 #pragma unroll
           for (int x = 0; x < 8; ++x) {
             const float2 v = make_float2(__uint_as_float(r[h][2 * x]), __uint_as_float(r[h][2 * x + 1]));
-            const float2 a = kWide ? __fmul2_rn(__fadd2_rn(v, from), c2) : __ffma2_rn(v, c2, less);
+            const float2 a = kWide ? __ffma2_rn(__fadd2_rn(v, from), c2, make_float2(kLift, kLift)) : __ffma2_rn(v, c2, less);
             const float2 e = make_float2(ex2(a.x), ex2(a.y));
             sum[x & 1] = __fadd2_rn(sum[x & 1], e);
             const __half2 q = __floats2half2_rn(e.x, e.y);

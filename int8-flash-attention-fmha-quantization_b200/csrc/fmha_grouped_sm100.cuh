@@ -22,6 +22,7 @@ namespace grouped {
 
 constexpr int kTile = 128;             // keys per tile
 constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23
+constexpr float kGrowth = 8.f;
 constexpr uint32_t kMagicBits = 0x4B400000u;
 
 struct Params {
@@ -44,7 +45,7 @@ struct Params {
   int few_rows;                        // 0, or: sequences with up to this many rows to a key head are the rows kernel's, the others the chunk kernel's
   long long first_unit;                // chunk kernel, units not split: those before this one are another launch's
   float c2;                            // from a difference of scores to an exponent of 2
-  int growth;                          // chunk kernel: a reference is kept while the maximum exceeds it by no more than this, 2^14 in p
+  int growth;                          // chunk kernel: a reference is kept while the maximum exceeds it by no more than this, 2^kGrowth in p
   float out_scale;                     // from sum p v / sum p, v in codes, to the output's unit
   unsigned* status;                    // eight device status words
   unsigned* host_word;                 // the host-visible failure word

@@ -12,7 +12,7 @@
 //     Up to four rows have four bytes each: 65535 e rounded down, and as many bits of what that leaves.  Up to eight have two, rn(65535 e), off by 2^-17 of the
 //     tile's largest e for every key however small its own is; where that may count, in a tile in which few keys have most of a row's weight, they have four too and
 //     there are two products.  (With 16 bits relative to the running maximum 131,072 keys behind one that lies 12.5 nats above them lost a third of their weight.);
-//   * up to sixteen rows P is fp16 and V becomes fp16 in registers (integers up to 2048 are exact there), m16n8k16;
+//   * up to sixteen rows P is fp16, 2^15 where p is 1, and V becomes fp16 in registers (integers up to 2048 are exact there), m16n8k16;
 //   * which key, column or row a lane's element belongs to is free as long as both operands agree, and is chosen so that each lane reads 16 bytes at a time
 //     without bank conflicts from the swizzled tiles, and so that the scores' registers are P's operand as they are;
 //   * the keys of a sequence are split over the warps of a cluster of CTAs, whose partial rows meet through distributed shared memory.
@@ -32,6 +32,8 @@ using namespace grouped;
 constexpr int kMaxCluster = 16;
 constexpr float kLevels = 65535.f;                   // of P in 16 bits
 constexpr uint32_t kCap = 2047u;                     // 2^-5 of them
+// Sixteen rows: P, sums and outputs are 2^15 times as large, so that the largest p still is an fp16 and the smallest step of one, 2^-24, is 2^-39 of it.
+constexpr float kHalfLift = 15.f;
 // 64 KB of tiles per CTA and three CTAs to an SM, or one CTA with three times as many warps
 template <int D> struct Cfg {
   static constexpr int kWarps = (D == 128) ? 2 : 4;
@@ -249,7 +251,8 @@ rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
     if constexpr (kWhole) ratio = most[0] == ref[0] ? 1.f : ex2((most[0] - ref[0]) * p.c2);
     auto power = [&](int h, int j) {
       const float to = kWhole ? most[h] : ref[h], base = to == -INFINITY ? 0.f : to;      // a row that sees no key: all e are zero
-      const float2 a = __fmul2_rn(__fadd2_rn(make_float2(x[h][j][0], x[h][j][1]), make_float2(-base, -base)), c2);
+      const float2 from_base = __fadd2_rn(make_float2(x[h][j][0], x[h][j][1]), make_float2(-base, -base));
+      const float2 a = kWhole ? __fmul2_rn(from_base, c2) : __ffma2_rn(from_base, c2, make_float2(kHalfLift, kHalfLift));
       return make_float2(ex2(a.x), ex2(a.y));
     };
     auto pack = [&](const float2& y) { return __byte_perm(__float_as_uint(y.x), __float_as_uint(y.y), 0x5410); };

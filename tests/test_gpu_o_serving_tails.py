@@ -56,7 +56,8 @@ def peaked(torch, tokens, keys, H, Hkv, D, nats, sinks, spread, value, seed):
 def bounded(torch, o, q, k, v, o_type, n_chain, what):
     """One sequence, causal.  In real units |o - exact| <=
       output   half a step of its type, relative
-      P        fp16 (more than eight rows): half a step, 2^-11 of p |v|; below 2^-14 of what it is relative to, 2^-25 of that, which is the row's largest p at most.
+      P        fp16 (more than eight rows): half a step, 2^-11 of p |v|; what it is relative to is 2^7 of fp16's units or more, so that the smallest half a step,
+               2^-25, is 2^-32 of that, which is the row's largest p at most.
                Up to eight rows, for each tile of 128 keys in which the row sees n: half a step of 16 bits, 2^-17 of the tile's largest p, for each of its keys where
                their p, none counted with more than 2^-5 of that, add up to n 2^-7 and more: 2^-10 of that sum times the mean |v|.  Half a step of 32 bits otherwise.
       exp2     2^-18 of every p, once above and once below the line of the quotient (as in _serving.tolerance)
@@ -75,7 +76,7 @@ def bounded(torch, o, q, k, v, o_type, n_chain, what):
         l = p.sum(-1, keepdim=True)
         want, each = p @ vv / l * real, p @ vv.abs() / l * real
         if n * G > 8:
-            of_p = each * 2.0 ** -11 + seen.double() @ vv.abs() / l * (2.0 ** -25 * real)
+            of_p = each * 2.0 ** -11 + seen.double() @ vv.abs() / l * (2.0 ** -32 * real)
         else:
             tiles = torch.nn.functional.pad(p, (0, -m % TILE)).view(n * G, -1, TILE)
             top = tiles.amax(-1, keepdim=True)
@@ -144,3 +145,28 @@ def test_the_same_row_in_any_company(pkg, torch, D):
         o = paged(pkg, torch, q[40 - n:], k, v, "fp16", keys)
         bounded(torch, o, q[40 - n:], k, v, "fp16", keys / 4, f"one of {n}")
         assert float((o[-1].double() - alone[0].double()).abs().max()) <= 2 * 2.0 ** -9 * float(alone.abs().max()), n
+
+
+# Sixteen rows, 32 in two groups, and the chunk kernel: whole units, and units shared by clusters.
+@pytest.mark.parametrize("D,H,Hkv,tokens", [(128, 4, 1, 4), (64, 16, 2, 1), (64, 8, 2, 8), (128, 12, 4, 40), (64, 6, 2, 70), (128, 8, 8, 300)])
+@pytest.mark.parametrize("keys,nats", [(8192, 12.5), (30000, 16.0), (30000, 18.5)])
+def test_more_rows_keep_what_a_dominant_key_leaves(pkg, torch, D, H, Hkv, tokens, keys, nats):
+    for sinks, value in (([0], 20), ([0, 1, 2, 3], 50), ([0, keys // 2 + 5], None)):
+        q, k, v = peaked(torch, tokens, keys, H, Hkv, D, nats, sinks, 0.5, value, seed=keys + D)
+        for most in (1, keys):
+            o = paged(pkg, torch, q, k, v, "bf16", most)
+            bounded(torch, o, q, k, v, "bf16", keys / 4, f"sinks {sinks}, values around {value}")
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_prompts_whose_largest_scores_come_late(pkg, torch, D):
+    """The reference of a row of the chunk kernel stays while the maximum exceeds it by less than 2^8: keys that grow by a little less and a little more than that, one by one and
+    tile by tile."""
+    c = scale_of(D)
+    for nats, gap in ((0.7, 1), (5.5, 128), (5.6, 128), (11.0, 300)):
+        q, k, v = peaked(torch, 200, 1500, 4, 2, D, 0.0, [], 0.3, 40, seed=D)
+        levels = ((torch.arange(1500, device="cuda") // gap) * (nats / (c * 127.0))).clamp(max=32 * 127).long()
+        for i in range(32):
+            k[:, :, i] = (levels // 32 + (i < levels % 32).long()).clamp(max=127).to(torch.int8)[:, None]
+        for most in (1, 1500):
+            bounded(torch, paged(pkg, torch, q, k, v, "bf16", most), q, k, v, "bf16", 1500 / 4, f"{nats} nats every {gap} keys")
