@@ -19,8 +19,8 @@
 //
 // 64 sequences of 1 to 8192 keys, 32 heads on 8 of 128: 105 us, 5.8 TB/s, 88 % of a copy's rate; 172 with P as fp16 (issue: 53 M instructions of six warps to an SM).  64 heads, eight
 // rows: 108, and 117 with two products in every tile.
-// One sequence of 1025 keys: 7.9 us, latencies in a row.  Two of 125,000 keys on 4 key heads, seven rows: 67 us on the 64 SMs that eight clusters
-// of eight have, 3.75 TB/s; 79 with scores of a deviation of 3, most of whose tiles need two products.
+// One sequence of 1025 keys: 7.9 us, latencies in a row.  Two of 125,000 keys on 4 key heads, seven rows: 64 us on the 64 SMs that eight clusters
+// of eight have, 3.9 TB/s; 76 with scores of a deviation of 3, most of whose tiles need two products.
 #pragma once
 #include "fmha_grouped_sm100.cuh"
 
@@ -131,13 +131,13 @@ rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
 
   const int g = lane >> 2, t4 = lane & 3, mine = kRows == 4 ? g & 3 : g;      // my row: g, one more of sixteen: g + 8, the same as lane - 16 of four
   uint32_t qa[kHalves][kWords];
-  int limit[kHalves], least = 0x7FFFFFFF;            // keys that my rows see, that all rows see
+  int limit[kHalves], least = 0x7FFFFFFF;            // keys that my rows see, that all rows see (a row that there is not is not stored)
 #pragma unroll
   for (int h = 0; h < kHalves; ++h) {
     const int row = row0 + mine + 8 * h, token = row / p.G;
     const bool real = row < n_rows;
     limit[h] = real ? visible(p, s, token) : 0;
-    least = min(least, limit[h]);
+    least = min(least, real ? limit[h] : 0x7FFFFFFF);
     const uint4* src = reinterpret_cast<const uint4*>(p.q + (s.q0 + token) * p.q_stride + (head * p.G + row - token * p.G) * D + t4 * (D / 4));
 #pragma unroll
     for (int c = 0; c < D / 64; ++c) {
