@@ -173,7 +173,8 @@ int fmha_i8_sm100_infer_host_slice(const float amax[5], const int desc[4],
  * which the work is divided; a longer sequence of keys is still computed in full, while tokens beyond max_seq_q may be left out (the device
  * status words say so: FMHA_I8_DEV_BAD_INDEX).  Offsets that point outside the tensors are cut to them and reported the same way.
  * max_seq_k, or what the tensors can hold where that is less, goes up to 2^30, and with more than 16 query rows to a key head (max_seq_q * head_num / head_num_kv) up
- * to 2^26: such a call with more may be refused with FMHA_I8_ERR_TOO_LARGE.
+ * to 2^26: such a call with more may be refused with FMHA_I8_ERR_TOO_LARGE, and where such a sequence has more keys than that, below a smaller bound, its tokens may be left as they were
+ * (reported the same way).
  * causal: token i of n_q sees keys j <= i + n_k - n_q, so that the last token sees all; without FMHA_I8_FLAG_CAUSAL all tokens see all keys.
  * q: int8, token t and head h at q + t * token stride + h * head_dim; o the same, int8 (requantised with amax[3] = o_amax), bf16 or fp16 (then
  * amax[3] is not looked at, nor is amax[4]).  All tensors 16-byte aligned, token strides in elements, whole multiples of 16 bytes.

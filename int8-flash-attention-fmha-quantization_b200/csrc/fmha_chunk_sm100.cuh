@@ -35,6 +35,9 @@ constexpr int kLaunchRegs = 128;
 constexpr int kSoftmaxRegs = 200, kConvertRegs = 56, kOtherRegs = 56;
 static_assert(2 * kSoftmaxRegs + kConvertRegs + kOtherRegs <= 4 * kLaunchRegs, "setmaxnreg targets exceed the CTA's register allocation: the kernel would hang");
 constexpr int kWarpConvert = 8, kWarpLoad = 12, kWarpScore = 13, kWarpWalk = 14, kWarpOutput = 15;
+// A warp may wait for a whole unit of another's, and gives up after about 1.5 s: 2^26 keys are 0.9 s.  Where a sequence has more, whatever bound the
+// call was given, its units are not walked.
+constexpr int kMostKeys = 1 << 26;
 constexpr int kInfos = 4;
 constexpr int kInfoConsumers = 8 + 4 + 1 + 2;      // softmax warps, converters, loader, issuers
 constexpr uint32_t kTmemCols = 512;
@@ -135,8 +138,9 @@ template <int D, bool kSplit> __device__ __forceinline__ void walk_role(const Pa
   auto pairs_of = [&](int b) {
     if (b >= p.B) return 0;
     const Seq s = load_seq(p, b);
-    if (!checked && (s.bad)) report(p.status, p.host_word, FMHA_I8_DEV_BAD_INDEX, 0u, b);
-    return s.nq * p.G <= p.few_rows ? 0 : (s.nq + 2 * p.tq - 1) / (2 * p.tq);
+    const bool ours = s.nq * p.G > p.few_rows, too_long = ours && s.nk > kMostKeys;
+    if (!checked && (s.bad || too_long)) report(p.status, p.host_word, FMHA_I8_DEV_BAD_INDEX, 0u, b);
+    return ours && !too_long ? (s.nq + 2 * p.tq - 1) / (2 * p.tq) : 0;
   };
   const int few = p.B <= 32 ? pairs_of(lane) : 0;   // up to 32 sequences: kept in registers
   for (uint32_t n = 0;; ++n) {

@@ -220,8 +220,6 @@ long long chunk_units(const grouped::Params& p) { return std::min<long long>(p.t
 // kernel's time (512 units of 1025 keys 38 and 62); head_dim 128 0.78 to 0.93 of it for 512 units and more of 1025 keys and more (4097 keys 174 and 223),
 // 1.02 to 1.54 for fewer or shorter ones.  33 to 48 rows: 0.60 to 1.08 and 1.05 to 1.22.
 constexpr int kMostGroup = 128;
-// A warp of the chunk kernel may wait for a whole unit of another's, and gives up after about 1.5 s: 2^26 keys are 0.9 s.
-constexpr long long kMostChunkKeys = 1LL << 26;
 bool few_rows(const Call& c, int sms) {
   const grouped::Params& p = c.p;
   const long long n_rows = static_cast<long long>(p.max_q) * p.G;
@@ -293,7 +291,7 @@ int run_attention(void* stream, Call& c) {
   c.p.status = dev.status;
   c.p.host_word = dev.host_word;
   const bool few = few_rows(c, dev.sm_count);
-  if (!few && c.max_k > kMostChunkKeys) return FMHA_I8_ERR_TOO_LARGE;
+  if (!few && c.max_k > chunk::kMostKeys) return FMHA_I8_ERR_TOO_LARGE;
   CUtensorMap mk, mv;
   if ((st = key_map(&mk, c.k, c.lk, c.D)) != FMHA_I8_OK) return st;
   if ((st = key_map(&mv, c.v, c.lv, c.D)) != FMHA_I8_OK) return st;
