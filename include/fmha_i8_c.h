@@ -17,7 +17,8 @@
  *             FMHA_I8_ERR_DEVICE by the first forward call made after the failing kernel has
  *             finished; that call launches nothing, the next one runs again.  The kernels
  *             themselves never look at the status words: one failure does not switch the
- *             library off.
+ *             library off.  What the serving calls find wrong in a caller's lengths, pages or
+ *             slots on the device is told by the status words alone and refuses no call.
  * All device-pointer entry points enqueue on the stream and return without synchronising.
  * Calls of the same shape give the same bytes every time.  A head's output may differ by 1 in a few elements of a million between
  * calls with different numbers of heads (slices, batches): the order of fp32 additions follows the division of the work.
@@ -43,7 +44,7 @@ enum {
   FMHA_I8_ERR_BAD_SLICE = -8,      /* bh_begin/bh_count outside [0, B*H] */
   FMHA_I8_ERR_BAD_AMAX = -9,       /* an amax is not a finite positive number */
   FMHA_I8_ERR_TOO_LARGE = -10,     /* size beyond a stated maximum of the entry point */
-  FMHA_I8_ERR_DEVICE = -11,        /* the device status words are non-zero (see device_status) */
+  FMHA_I8_ERR_DEVICE = -11,        /* a wait in an earlier kernel ran out; of device_status: its words are non-zero */
   FMHA_I8_ERR_BAD_FLAGS = -12      /* a flag bit this library does not define is set */
 };
 
@@ -63,8 +64,8 @@ enum {
   FMHA_I8_DEV_WAIT_INFO = 11,      /* a role waiting for (or the scanner waiting to reuse) a unit's mask information */
   FMHA_I8_DEV_WAIT_QUANT = 12,     /* quantiser: a tile of the tensor */
   FMHA_I8_DEV_WAIT_S_FREE = 14,    /* MMA issuer waiting for the scores before to be read */
-  /* No wait, but an index in device memory that points outside its tensor (nothing was accessed there): words[2] = 0: lengths or offsets of
-   * sequence words[3]; 1: a page of sequence words[3]; 2: position or slot of token words[3]. */
+  /* No wait, but an index in device memory that points outside its tensor (nothing was accessed there), or a length beyond what the call allows: words[2] = 0: lengths or
+   * offsets of sequence words[3]; 1: a page of sequence words[3]; 2: position or slot of token words[3].  No later call is refused for it. */
   FMHA_I8_DEV_BAD_INDEX = 13
 };
 
@@ -296,7 +297,8 @@ int fmha_i8_sm100_debug_quantize_whole_chip(void* stream, const float* x, long l
 /* Synchronises the current device, copies out and clears the eight device status words.
  * words[0] == 0 means no kernel of this library gave up on a bounded wait since the last call.
  * Otherwise words[0] = which wait gave up (FMHA_I8_DEV_*), words[1] = block index, words[2] = warp,
- * words[3] = key-tile counter of the first failure.
+ * words[3] = key-tile counter of the first failure.  words[4..7] = the same of the first index
+ * outside its tensor (FMHA_I8_DEV_BAD_INDEX), and words[0..3] too where no wait ran out.
  * Returns FMHA_I8_OK, FMHA_I8_ERR_DEVICE when words[0] != 0, or FMHA_I8_ERR_LAUNCH. */
 int fmha_i8_sm100_device_status(unsigned words[8]);
 

@@ -1061,6 +1061,8 @@ int fmha_i8_sm100_device_status(unsigned words[8]) {
       if (g_dev[dev_id].host_flag) *g_dev[dev_id].host_flag = 0u;
     }
   }
+  if (words[0] == 0u)
+    for (int i = 0; i < 4; ++i) words[i] = words[4 + i];
   return finish(words[0] == 0u ? FMHA_I8_OK : FMHA_I8_ERR_DEVICE);
 }
 
@@ -1079,7 +1081,7 @@ const char* fmha_i8_sm100_status_string(int status) {
     case FMHA_I8_ERR_BAD_SLICE: return "bh_begin/bh_count outside the batch*head range";
     case FMHA_I8_ERR_BAD_AMAX: return "amax values must be finite and positive";
     case FMHA_I8_ERR_TOO_LARGE: return "size beyond the maximum of this entry point";
-    case FMHA_I8_ERR_DEVICE: return "a device-side bounded wait ran out or an index pointed outside its tensor (see fmha_i8_sm100_device_status)";
+    case FMHA_I8_ERR_DEVICE: return "a device-side bounded wait ran out, or (device_status only) an index pointed outside its tensor (see fmha_i8_sm100_device_status)";
     case FMHA_I8_ERR_BAD_FLAGS: return "an undefined flag bit is set";
     default: return "unknown status";
   }

@@ -139,7 +139,7 @@ template <int D, bool kSplit> __device__ __forceinline__ void walk_role(const Pa
     if (b >= p.B) return 0;
     const Seq s = load_seq(p, b);
     const bool ours = s.nq * p.G > p.few_rows, too_long = ours && s.nk > kMostKeys;
-    if (!checked && (s.bad || too_long)) report(p.status, p.host_word, FMHA_I8_DEV_BAD_INDEX, 0u, b);
+    if (!checked && (s.bad || too_long)) report_index(p.status, 0u, b);
     return ours && !too_long ? (s.nq + 2 * p.tq - 1) / (2 * p.tq) : 0;
   };
   const int few = p.B <= 32 ? pairs_of(lane) : 0;   // up to 32 sequences: kept in registers
@@ -249,7 +249,7 @@ template <int D> __device__ __forceinline__ void load_role(const Params& p, Ctl<
       }
       page = next_page;
     }
-    if (bad_page) report(p.status, p.host_word, FMHA_I8_DEV_BAD_INDEX, 1u, u.b);
+    if (bad_page) report_index(p.status, 1u, u.b);
     __syncwarp();
   }
 }

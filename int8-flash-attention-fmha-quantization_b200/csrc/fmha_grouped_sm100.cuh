@@ -51,7 +51,7 @@ struct Params {
   unsigned* host_word;                 // the host-visible failure word
 };
 
-// Records what went wrong first: words {code, block, detail0, detail1}, and tells the host.
+// Records which wait ran out first: words {code, block, detail0, detail1}, and tells the host.
 __device__ __noinline__ void report(unsigned* status, unsigned* host_word, unsigned code, unsigned detail0, unsigned detail1) {
   if (atomicCAS(&status[0], 0u, code) == 0u) {
     status[1] = blockIdx.x;
@@ -61,6 +61,15 @@ __device__ __noinline__ void report(unsigned* status, unsigned* host_word, unsig
       *reinterpret_cast<volatile unsigned*>(host_word) = 1u;
       __threadfence_system();
     }
+  }
+}
+
+// Records an index that points outside its tensor, in the words behind: that is one caller's data, the output of others is right, so it hides no failure and the host is not told.
+__device__ __noinline__ void report_index(unsigned* status, unsigned detail0, unsigned detail1) {
+  if (atomicCAS(&status[4], 0u, static_cast<unsigned>(FMHA_I8_DEV_BAD_INDEX)) == 0u) {
+    status[5] = blockIdx.x;
+    status[6] = detail0;
+    status[7] = detail1;
   }
 }
 

@@ -18,7 +18,7 @@ namespace fmha {
 namespace rope {
 
 using grouped::kMagic;
-using grouped::report;
+using grouped::report_index;
 
 constexpr int kThreads = 128;
 
@@ -37,7 +37,6 @@ struct Params {
   int parts;                           // warps per token
   float amax[3], scale[3];             // ranges of q, k, v, and 127 / range
   unsigned* status;
-  unsigned* host_word;
 };
 
 // Eight neighbouring elements as they are in memory, and as four pairs of floats.
@@ -197,7 +196,7 @@ __global__ void __launch_bounds__(kThreads, 5) append_kernel(const Params p) {
   };
   if (head0 < stop) load(head0, a, b);
   const bool no_position = position < 0 || position >= p.in_table, no_slot = p.slots != nullptr && slot >= p.num_slots;
-  if ((no_position || no_slot) && lane == 0 && part == 0) report(p.status, p.host_word, FMHA_I8_DEV_BAD_INDEX, 2u, token);
+  if ((no_position || no_slot) && lane == 0 && part == 0) report_index(p.status, 2u, token);
   if (no_position) return;
   if (no_slot) slot = -1;
   Turn turn;

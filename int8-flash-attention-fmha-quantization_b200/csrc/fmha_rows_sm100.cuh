@@ -122,7 +122,7 @@ rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
   const int head = unit % p.Hkv, b = unit / p.Hkv;
   const Seq s = load_seq(p, b);
   // (of a mixed batch the chunk kernel computes sequences longer than the bound in full)
-  if (threadIdx.x == 0 && rank == 0 && group == 0 && head == 0 && (s.bad || (s.nq > p.max_q && p.few_rows == 0))) report(p.status, p.host_word, FMHA_I8_DEV_BAD_INDEX, 0u, b);
+  if (threadIdx.x == 0 && rank == 0 && group == 0 && head == 0 && (s.bad || (s.nq > p.max_q && p.few_rows == 0))) report_index(p.status, 0u, b);
   const int n_rows = s.nq * p.G, row0 = group * kRows;
   if (row0 >= n_rows || (p.few_rows != 0 && n_rows > p.few_rows)) return;      // the whole cluster
   const int end = visible(p, s, min(row0 + kRows - 1, n_rows - 1) / p.G);      // the last token of the group sees most
@@ -402,7 +402,7 @@ rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
     }
     __syncwarp();
   }
-  if (bad_page) report(p.status, p.host_word, FMHA_I8_DEV_BAD_INDEX, 1u, b);
+  if (bad_page) report_index(p.status, 1u, b);
 
   // ---- the warp's partial rows go over its own tiles, which it has done with
 #pragma unroll

@@ -413,7 +413,6 @@ int append_impl(void* stream, const float amax[5], const long long dims[5], cons
   int st = fmha_host::device_for_call(&dev);
   if (st != FMHA_I8_OK || tokens == 0) return st;
   p.status = dev.status;
-  p.host_word = dev.host_word;
   // Warps that take one round of heads each, up to 48 warps to an SM, then more rounds.  8192 tokens of 48 heads of 128: 42.9 us; with 96 warps 47.2, 160 53.4, 320 54.7 (a
   // warp's later rounds have the table's entries and the position already, and the next heads on their way).
   const int at_once = static_cast<int>(512 / D), all = static_cast<int>((H + 2 * Hkv + at_once - 1) / at_once);

@@ -47,3 +47,62 @@ def test_a_chunk_on_more_keys_than_waits_are_sized_for_below_a_smaller_bound(pkg
         want, scales = attention64(q[at:at + n], k, v, AMAX, True)
         check(o[at:at + n], want, scales, m, "bf16", AMAX, 1.0, max_q * H // 2, f"sequence {b}", own=n * H // 2)
         at += n
+
+
+def small_forward(pkg, torch):
+    """A padded forward call: what it gives, as a function, and the arguments."""
+    q, k, v = (codes((1, 2, 128, 64), s) for s in (11, 12, 13))
+    mask = torch.zeros((1, 128), dtype=torch.int8, device="cuda")
+    return lambda o, check=True: pkg.FMHAInferI8(None, pkg.FMHAParamI8(*AMAX, 1.0, 1.0), pkg.AttnDataDescriptor(1, 128, 2, 64), q, k, v, mask, o, True, check=check)
+
+
+def bad_calls(pkg, torch):
+    """A page, a length, an offset and a slot that point outside their tensors, one call each: its code and the detail that is reported."""
+    kc, vc = codes((4, 1, 16, 64), 1), codes((4, 1, 16, 64), 2)
+    q, o = codes((2, 1, 64), 3), torch.empty((2, 1, 64), dtype=torch.bfloat16, device="cuda")
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    desc = pkg.AttnDataDescriptorGrouped(2, 1, 32, 1, 1, 64)
+    x = torch.zeros((2, 1, 64), device="cuda")
+    codes_out = codes((2, 1, 64), 4)
+    return [(lambda: pkg.FMHAInferI8Paged(None, param(pkg), desc, q, kc, vc, i32(0, 9, 1, 2).view(2, 2), i32(20, 20), starts([1, 1]), o), 1, 0),
+            (lambda: pkg.FMHAInferI8Paged(None, param(pkg), desc, q, kc, vc, i32(0, 3, 1, 2).view(2, 2), i32(20, 33), starts([1, 1]), o), 0, 1),
+            (lambda: pkg.FMHAInferI8Packed(None, param(pkg), desc, q, q, q, i32(0, 1, 3), i32(0, 1, 2), o), 0, 1),
+            (lambda: pkg.rope_quantize_append(None, param(pkg), x, x, x, i32(0, 0), None, codes_out, kc, vc, slots=torch.tensor([0, 64], device="cuda")), 2, 1)]
+
+
+def test_an_index_outside_is_nobody_elses_error(pkg, torch):
+    """It is reported through the status words alone: the next calls run, whoever makes them."""
+    forward = small_forward(pkg, torch)
+    want = torch.empty((1, 2, 128, 64), dtype=torch.int8, device="cuda")
+    forward(want)
+    for call, detail, which in bad_calls(pkg, torch):
+        call()
+        torch.cuda.synchronize()
+        o = torch.zeros_like(want)
+        forward(o)
+        assert torch.equal(o, want)
+        q, k, v = codes((5, 2, 64), 1), codes((5, 2, 64), 2), codes((5, 2, 64), 3)
+        got = torch.empty((5, 2, 64), dtype=torch.bfloat16, device="cuda")
+        cu = starts([5])
+        pkg.FMHAInferI8Packed(None, param(pkg), pkg.AttnDataDescriptorGrouped(1, 5, 5, 2, 2, 64), q, k, v, cu, cu, got)
+        exact, scales = attention64(q, k, v, AMAX, True)
+        check(got, exact, scales, 5, "bf16", AMAX, 1.0, 5)
+        st, words = pkg.device_status()
+        assert st == pkg.ERR_DEVICE and words[0] == DEV_BAD_INDEX and words[2:4] == [detail, which], words
+        assert pkg.device_status()[0] == pkg.OK
+
+
+def test_an_index_outside_hides_no_wait_that_ran_out(pkg, torch):
+    forward = small_forward(pkg, torch)
+    o = torch.empty((1, 2, 128, 64), dtype=torch.int8, device="cuda")
+    forward(o)
+    call, detail, which = bad_calls(pkg, torch)[0]
+    call()
+    torch.cuda.synchronize()
+    pkg.debug_wait_probe(None, 4_000_000)                 # a kernel that waits two milliseconds for nothing
+    torch.cuda.synchronize()
+    forward(o, check=False)
+    assert pkg.lib().fmha_i8_sm100_last_status() == pkg.ERR_DEVICE
+    st, words = pkg.device_status()
+    assert st == pkg.ERR_DEVICE and words[0] == 10 and words[4] == DEV_BAD_INDEX and words[6:8] == [detail, which], words
+    forward(o)
