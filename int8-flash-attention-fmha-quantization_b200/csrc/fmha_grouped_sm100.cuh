@@ -107,7 +107,7 @@ __device__ __forceinline__ Seq load_seq(const Params& p, int b) {
 }
 // Keys that token t of the sequence sees: the first visible(...) of them.
 __device__ __forceinline__ int visible(const Params& p, const Seq& s, int t) {
-  return p.causal ? min(max(t + 1 + s.nk - s.nq, 0), s.nk) : s.nk;
+  return p.causal ? min(max(t + 1 - s.nq + s.nk, 0), s.nk) : s.nk;
 }
 
 // The copies that bring keys [key0, key0 + 128) of sequence b: copy i (lane i of the warp that calls this) brings 2^box_shift of them.  `page`

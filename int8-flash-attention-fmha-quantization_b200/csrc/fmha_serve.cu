@@ -25,6 +25,11 @@ using fmha_host::finish;
 constexpr int kMaxDevices = 64;
 constexpr long long kMostRows = 0x7FFFFFFFLL;
 
+// n rows (or pages) `stride` elements apart lie in no memory: a stride that a tensor map cannot hold, or a span beyond all addresses.
+bool too_far(long long n, long long stride, int bytes) {
+  constexpr long long kMostStride = 1LL << 40, kMostSpan = 1LL << 47;
+  return stride >= kMostStride / bytes || (n > 0 && stride * bytes > kMostSpan / n);
+}
 bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 bool power_of_two(long long n) { return n > 0 && (n & (n - 1)) == 0; }
 int log2_of(long long n) { int s = 0; while ((1LL << s) < n) ++s; return s; }
@@ -160,7 +165,8 @@ int fill_call(Call* c, const float amax[5], const int desc6[6], const void* q, c
   if (o_type != FMHA_I8_TYPE_I8 && o_type != FMHA_I8_TYPE_BF16 && o_type != FMHA_I8_TYPE_FP16) return FMHA_I8_ERR_BAD_SHAPE;
   if (total_q < 0 || q_stride < static_cast<long long>(H) * D || o_stride < static_cast<long long>(H) * D) return FMHA_I8_ERR_BAD_SHAPE;
   const int G = H / Hkv;
-  if (total_q * H > kMostRows || static_cast<long long>(max_q) * G > kMostRows - 256 || max_k > (1 << 30)) return FMHA_I8_ERR_TOO_LARGE;
+  if (total_q > kMostRows / H || static_cast<long long>(max_q) * G > kMostRows - 256 || max_k > (1 << 30) || static_cast<long long>(B) * Hkv > kMostRows) return FMHA_I8_ERR_TOO_LARGE;
+  if (too_far(total_q, q_stride, 1) || too_far(total_q, o_stride, type_bytes(o_type))) return FMHA_I8_ERR_TOO_LARGE;
   if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(o, 16) || !aligned(cu_q, 4)) return FMHA_I8_ERR_MISALIGNED;
   if (q_stride % 16 != 0 || o_stride * type_bytes(o_type) % 16 != 0) return FMHA_I8_ERR_MISALIGNED;
   for (int i = 0; i < (o_type == FMHA_I8_TYPE_I8 ? 4 : 3); ++i)
@@ -196,7 +202,7 @@ template <int D, int kRows> int launch_rows(cudaStream_t stream, const Device& d
   p.row_groups = p.few_rows != 0 ? 1 : static_cast<int>((static_cast<long long>(p.max_q) * p.G + kRows - 1) / kRows);
   const long long units = static_cast<long long>(p.B) * p.Hkv * p.row_groups;
   const long long n_tiles = (c.max_k + grouped::kTile - 1) / grouped::kTile;
-  if (units > kMostRows / rows::kMaxCluster) return FMHA_I8_ERR_TOO_LARGE;
+  if (units > kMostRows / rows::kMaxCluster) return FMHA_I8_ERR_TOO_LARGE;      // (B * Hkv is below 2^31, and the groups below 2^29)
   const long long resident = 3LL * dev.sm_count;
   // Few units with many keys: one CTA with all the warps of an SM on as many SMs as a cluster allows.  8 units of 131,072 keys, head_dim 128: 63 us; the CTAs of
   // two warps below in clusters of 8 74, of 16 67 to 76.
@@ -314,7 +320,7 @@ int infer_packed_impl(void* stream, const float amax[5], const int desc6[6], con
   if (st != FMHA_I8_OK) return st;
   const long long width = static_cast<long long>(c.p.Hkv) * c.D;
   if (tokens[1] < 0 || strides[1] < width || strides[2] < width) return FMHA_I8_ERR_BAD_SHAPE;
-  if (tokens[1] > (1LL << 30)) return FMHA_I8_ERR_TOO_LARGE;
+  if (tokens[1] > (1LL << 30) || too_far(tokens[1], strides[1], 1) || too_far(tokens[1], strides[2], 1)) return FMHA_I8_ERR_TOO_LARGE;
   if (strides[1] % 16 != 0 || strides[2] % 16 != 0 || !aligned(cu_k, 4)) return FMHA_I8_ERR_MISALIGNED;
   c.p.cu_k = cu_k;
   c.p.total_k = static_cast<int>(tokens[1]);
@@ -336,7 +342,7 @@ int infer_paged_impl(void* stream, const float amax[5], const int desc6[6], cons
   if (st != FMHA_I8_OK) return st;
   const long long pages = cache[0], page = cache[1], page_stride = cache[2], width = cache[3], table_stride = cache[4];
   if (pages < 1 || !power_of_two(page) || page < 16 || page > 4096 || page_stride < c.p.Hkv * page * c.D || width < 1 || table_stride < width) return FMHA_I8_ERR_BAD_SHAPE;
-  if (pages > 0x7FFFFFFELL || width > ((1LL << 30) / page)) return FMHA_I8_ERR_TOO_LARGE;
+  if (pages > 0x7FFFFFFELL || width > ((1LL << 30) / page) || too_far(pages, page_stride, 1) || too_far(c.p.B, table_stride, 4)) return FMHA_I8_ERR_TOO_LARGE;
   if (page_stride % 16 != 0 || !aligned(page_table, 4) || !aligned(lens_k, 4)) return FMHA_I8_ERR_MISALIGNED;
   c.p.lens_k = lens_k;
   c.p.page_table = page_table;
@@ -380,8 +386,11 @@ int append_impl(void* stream, const float amax[5], const long long dims[5], cons
   if (tokens < 0 || H < 1 || Hkv < 1 || (D != 64 && D != 128) || rot < 0 || rot > D || rot % 16 != 0) return FMHA_I8_ERR_BAD_SHAPE;
   if (in_type != FMHA_I8_TYPE_BF16 && in_type != FMHA_I8_TYPE_FP16 && in_type != FMHA_I8_TYPE_FP32) return FMHA_I8_ERR_BAD_SHAPE;
   if (rot > 0 && !table) return FMHA_I8_ERR_NULL_POINTER;
+  if (H > 65536 || Hkv > 65536) return FMHA_I8_ERR_TOO_LARGE;
   if (in_table < 0 || strides[0] < H * D || strides[1] < Hkv * D || strides[2] < Hkv * D) return FMHA_I8_ERR_BAD_SHAPE;
-  if (H > 65536 || Hkv > 65536 || tokens * (H + 2 * Hkv) > kMostRows || in_table > kMostRows) return FMHA_I8_ERR_TOO_LARGE;
+  if (tokens > kMostRows / (H + 2 * Hkv) || in_table > kMostRows) return FMHA_I8_ERR_TOO_LARGE;
+  for (int i = 0; i < 3; ++i)
+    if (too_far(tokens, strides[i], type_bytes(in_type))) return FMHA_I8_ERR_TOO_LARGE;
   for (int i = 0; i < 3; ++i)
     if (!(amax[i] > 0.f) || !std::isfinite(amax[i]) || !std::isfinite(127.f / amax[i])) return FMHA_I8_ERR_BAD_AMAX;
   const int bytes = type_bytes(in_type);
@@ -391,7 +400,7 @@ int append_impl(void* stream, const float amax[5], const long long dims[5], cons
   rope::Params p{};
   if (slots) {
     if (cache[0] < 1 || !power_of_two(cache[1]) || cache[1] < 16 || cache[1] > 4096 || cache[2] < Hkv * cache[1] * D) return FMHA_I8_ERR_BAD_SHAPE;
-    if (cache[0] > 0x7FFFFFFELL) return FMHA_I8_ERR_TOO_LARGE;
+    if (cache[0] > 0x7FFFFFFELL || too_far(cache[0], cache[2], 1)) return FMHA_I8_ERR_TOO_LARGE;
     if (cache[2] % 16 != 0) return FMHA_I8_ERR_MISALIGNED;
     p.page_shift = log2_of(cache[1]);
     p.page_stride = cache[2];
