@@ -199,7 +199,8 @@ int fill_call(Call* c, const float amax[5], const int desc6[6], const void* q, c
 template <int D, int kRows> int launch_rows(cudaStream_t stream, const Device& dev, Call& c, const CUtensorMap& mk, const CUtensorMap& mv) {
   grouped::Params& p = c.p;
   constexpr int W = RowsCfg<D>::kWarps, Wide = RowsCfg<D>::kWarpsWide;
-  p.row_groups = p.few_rows != 0 ? 1 : static_cast<int>((static_cast<long long>(p.max_q) * p.G + kRows - 1) / kRows);
+  // (one at least: a sequence with tokens where the call allows none is to be reported)
+  p.row_groups = p.few_rows != 0 ? 1 : std::max(1, static_cast<int>((static_cast<long long>(p.max_q) * p.G + kRows - 1) / kRows));
   const long long units = static_cast<long long>(p.B) * p.Hkv * p.row_groups;
   const long long n_tiles = (c.max_k + grouped::kTile - 1) / grouped::kTile;
   if (units > kMostRows / rows::kMaxCluster) return FMHA_I8_ERR_TOO_LARGE;      // (B * Hkv is below 2^31, and the groups below 2^29)
@@ -293,7 +294,7 @@ int run_attention(void* stream, Call& c) {
   int st;
   if ((st = fmha_host::device_for_call(&dev)) != FMHA_I8_OK) return st;
   if ((st = set_up(dev)) != FMHA_I8_OK) return st;
-  if (c.p.total_q == 0 || c.p.max_q == 0) return FMHA_I8_OK;
+  if (c.p.total_q == 0) return FMHA_I8_OK;
   c.p.status = dev.status;
   c.p.host_word = dev.host_word;
   const bool few = few_rows(c, dev.sm_count);

@@ -106,3 +106,23 @@ def test_an_index_outside_hides_no_wait_that_ran_out(pkg, torch):
     st, words = pkg.device_status()
     assert st == pkg.ERR_DEVICE and words[0] == 10 and words[4] == DEV_BAD_INDEX and words[6:8] == [detail, which], words
     forward(o)
+
+
+@pytest.mark.parametrize("D,H", [(64, 4), (128, 48)])
+def test_tokens_where_the_call_allows_none_are_reported(pkg, torch, D, H):
+    """max_seq_q = 0 with tokens on the device: they may be left as they were, but not without a word.  Without tokens there is nothing to say."""
+    q, k = codes((5, H, D), 1), codes((5, 2, D), 2)
+    o = torch.full((5, H, D), 7.0, dtype=torch.bfloat16, device="cuda")
+    desc = pkg.AttnDataDescriptorGrouped(2, 0, 5, H, 2, D)
+    lens, table = torch.tensor([3, 2], dtype=torch.int32, device="cuda"), torch.zeros((2, 1), dtype=torch.int32, device="cuda")
+    kc = codes((1, 2, 16, D), 3)
+    for tokens in (starts([0, 3]), starts([3, 2]), starts([0, 0])):
+        for call in (lambda: pkg.FMHAInferI8Packed(None, param(pkg), desc, q, k, k, tokens, starts([2, 3]), o),
+                     lambda: pkg.FMHAInferI8Paged(None, param(pkg), desc, q, kc, kc, table, lens, tokens, o)):
+            call()
+            st, words = pkg.device_status()
+            if int(tokens[-1]) == 0:
+                assert st == pkg.OK and bool((o == 7.0).all())
+            else:
+                assert st == pkg.ERR_DEVICE and words[0] == DEV_BAD_INDEX and words[2] == 0, words
+            o.fill_(7.0)
