@@ -213,8 +213,8 @@ int fmha_i8_sm100_rope_table(void* stream, const double* inv_freq, int pairs, lo
  *              in fmha_i8_sm100_infer_paged, and token t goes to page slot / page_size, place slot % page_size; a negative slot is not stored.  Two
  *              tokens with the same slot leave a mixture of both there.
  * dims[5] = {tokens, head_num, head_num_kv, head_dim, rot_dim}; strides[3] = those of q, k, v; positions_in_table; cache[3] = {num_pages, page_size,
- * page_stride} (not looked at without slots).  A token whose position lies outside the table is left out, and a slot outside the cache is
- * not stored; both are reported through the device status words.  No tokens: nothing happens. */
+ * page_stride} (not looked at without slots).  A token whose position lies outside the table is left out (without a rotation positions are not looked at), and a slot outside the
+ * cache is not stored; both are reported through the device status words.  No tokens: nothing happens. */
 int fmha_i8_sm100_rope_quantize_append(void* stream, const float amax[5], const long long dims[5], const void* q, const void* k, const void* v, int in_type,
                                        const long long strides[3], const int* positions, const float* table, long long positions_in_table,
                                        int interleaved, int8_t* q_out, int8_t* k_out, int8_t* v_out, const long long* slots, const long long cache[3]);

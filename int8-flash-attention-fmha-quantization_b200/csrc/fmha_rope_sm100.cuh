@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(kThreads, 5) append_kernel(const Params p) {
     load8(in + (apart ? half + 8 * l : 16 * l + 8), y);
   };
   if (head0 < stop) load(head0, a, b);
-  const bool no_position = position < 0 || position >= p.in_table, no_slot = p.slots != nullptr && slot >= p.num_slots;
+  const bool no_position = p.rot > 0 && (position < 0 || position >= p.in_table), no_slot = p.slots != nullptr && slot >= p.num_slots;
   if ((no_position || no_slot) && lane == 0 && part == 0) report_index(p.status, 2u, token);
   if (no_position) return;
   if (no_slot) slot = -1;

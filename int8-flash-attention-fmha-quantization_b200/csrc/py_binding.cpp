@@ -457,11 +457,9 @@ PyObject* py_rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (T == 0) return PyLong_FromLong(0);
   const long long rot = turned ? table.size[2] : 0;
   const long long shape[5] = {T, H, Hkv, D, rot}, strides[3] = {outer_stride(q), outer_stride(k), outer_stride(v)}, cache[3] = {k_out.size[0], paged ? k_out.size[2] : 0, outer_stride(k_out)};
-  // without a rotation any position will do
-  const long long in_table = rot > 0 ? table.size[1] : 0x7FFFFFFFLL;
   Py_BEGIN_ALLOW_THREADS
   st = fmha_i8_sm100_rope_quantize_append(stream, amax, shape, q.ptr, k.ptr, v.ptr, q.type, strides, static_cast<const int*>(positions.ptr),
-                                          static_cast<const float*>(table.ptr), in_table, interleaved, static_cast<int8_t*>(q_out.ptr), static_cast<int8_t*>(k_out.ptr),
+                                          static_cast<const float*>(table.ptr), turned ? table.size[1] : 0, interleaved, static_cast<int8_t*>(q_out.ptr), static_cast<int8_t*>(k_out.ptr),
                                           static_cast<int8_t*>(v_out.ptr), static_cast<const long long*>(slots.ptr), cache);
   Py_END_ALLOW_THREADS
   return PyLong_FromLong(st);

@@ -126,3 +126,22 @@ def test_tokens_where_the_call_allows_none_are_reported(pkg, torch, D, H):
             else:
                 assert st == pkg.ERR_DEVICE and words[0] == DEV_BAD_INDEX and words[2] == 0, words
             o.fill_(7.0)
+
+
+@pytest.mark.parametrize("page", [0, 16])
+def test_without_a_rotation_any_position_will_do(pkg, torch, page):
+    """No table, no positions to look up: tokens with positions below zero and far out are quantised and stored like the others, and nothing is reported."""
+    T, H, Hkv, D = 6, 3, 1, 64
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1)
+    q, k, v = (torch.randn((T, h, D), device="cuda", generator=g).bfloat16() for h in (H, Hkv, Hkv))
+    outs = []
+    for positions in ([0, 1, 2, 3, 4, 5], [-1, 2 ** 31 - 1, -2 ** 31, 7, -5, 0]):
+        q_out = torch.zeros((T, H, D), dtype=torch.int8, device="cuda")
+        ko, vo = (torch.zeros((1, Hkv, page, D) if page else (T, Hkv, D), dtype=torch.int8, device="cuda") for _ in range(2))
+        pkg.rope_quantize_append(None, param(pkg), q, k, v, torch.tensor(positions, dtype=torch.int32, device="cuda"), None, q_out, ko, vo,
+                                 slots=torch.arange(T, device="cuda") if page else None)
+        outs.append((q_out, ko, vo))
+        st, words = pkg.device_status()
+        assert st == pkg.OK, words
+    assert all(torch.equal(a, b) for a, b in zip(*outs)) and bool(outs[0][1].any())
