@@ -209,7 +209,7 @@ int set_kernel_attributes(DeviceInfo* d) {
 
 // Driver entry points, fetched through the runtime so the library has no link-time libcuda dependency.
 using fmha_host::EncodeTiledFn;
-using fmha_host::ReplaceAddressFn;
+using ReplaceAddressFn = CUresult (*)(CUtensorMap*, void*);
 using PointerAttributeFn = CUresult (*)(void*, CUpointer_attribute, CUdeviceptr);
 template <typename Fn> Fn driver_fn(const char* name) {
   void* f = nullptr;
@@ -730,8 +730,6 @@ int device_for_call(Device* out) {
 void count_launch() { g_launch_count.fetch_add(1, std::memory_order_relaxed); }
 
 EncodeTiledFn encode_tiled() { return encode_fn(); }
-
-ReplaceAddressFn replace_address() { return replace_address_fn(); }
 
 }  // namespace fmha_host
 

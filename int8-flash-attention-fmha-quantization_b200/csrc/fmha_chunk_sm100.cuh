@@ -516,18 +516,15 @@ template <int D, bool kWide, bool kSplit> __device__ __forceinline__ void softma
         for (int h = 0; h < 8; ++h) {
           if (h == 4 && grew) {
             // The reference has moved: what has been summed so far is rescaled before more is added.  (The scores of this step were formed behind P.V of the one
-            // before.)  Here, where half of the scores have become powers, there are registers for 32 columns at a time.
+            // before.)  Here, where half of the scores have become powers, there are registers for 16 columns.
 #pragma unroll 1
             for (int x = 0; x < D; x += 16) {
-              uint32_t o[1][16];
-              tmem_ld16_issue(tO + x, o[0]);
+              uint32_t o[16];
+              tmem_ld16_issue(tO + x, o);
+              tmem_ld_fence(o);
 #pragma unroll
-              for (int z = 0; z < 1; ++z) {
-                tmem_ld_fence(o[z]);
-#pragma unroll
-                for (int y = 0; y < 16; ++y) o[z][y] = __float_as_uint(__uint_as_float(o[z][y]) * factor);
-                tmem_st16(tO + x + 16 * z, o[z]);
-              }
+              for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * factor);
+              tmem_st16(tO + x, o);
             }
           }
           uint32_t packed[8];

@@ -40,7 +40,7 @@ struct Params {
   int total_q, total_k, max_q;
   int o_type, causal;
   int o_wide;                          // rows of o are 32-byte aligned
-  int row_groups;                      // rows kernel: groups of 16 rows per sequence and key head
+  int row_groups;                      // rows kernel: groups of 4, 8 or 16 rows per sequence and key head
   int tq;                              // chunk kernel: tokens per tile of 128 rows
   int few_rows;                        // 0, or: sequences with up to this many rows to a key head are the rows kernel's, the others the chunk kernel's
   long long first_unit;                // chunk kernel, units not split: those before this one are another launch's

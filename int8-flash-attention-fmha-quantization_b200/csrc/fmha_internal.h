@@ -9,7 +9,6 @@ namespace fmha_host {
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                    const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                    CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-using ReplaceAddressFn = CUresult (*)(CUtensorMap*, void*);
 
 struct Device {
   int index = 0, sm_count = 1;
@@ -23,7 +22,6 @@ int finish(int status);
 int device_for_call(Device* out);
 void count_launch();
 EncodeTiledFn encode_tiled();
-ReplaceAddressFn replace_address();
 
 }  // namespace fmha_host
 #pragma GCC visibility pop

@@ -1,7 +1,7 @@
 // Attention of a few query rows per key head over packed or paged sequences with grouped heads: single new tokens against a cache.
 // The formulas are in fmha_grouped_sm100.cuh.
 //
-// The G heads of a group and the new tokens of a sequence make the rows: row r is token r / G, head r % G of the group, sixteen at a time.
+// The G heads of a group and the new tokens of a sequence make the rows: row r is token r / G, head r % G of the group, four, eight or sixteen at a time.
 // What bounds it: K and V of a key head are read once for all of a group's rows, so HBM does, 2 D bytes per key.  A tensor-core tile of
 // tcgen05.mma has 128 rows; here eight or sixteen are enough, so the products are warp-level ones, and
 //   * a warp owns whole tiles of 128 keys, with its running maximum, sum and output rows in registers; it asks for its next K
