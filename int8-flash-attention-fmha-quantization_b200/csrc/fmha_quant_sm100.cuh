@@ -33,11 +33,14 @@ __device__ __forceinline__ int quant_one(float v, float scale) {
 // finite: false is returned if it may not be, and the words are then quant_one's to make.
 template <int N>
 __device__ __forceinline__ bool quant_words(const float4 (&v)[N], float scale, uint32_t (&words)[N]) {
-  const float2 s2 = make_float2(scale, scale), half = make_float2(0.5f, 0.5f), magic = make_float2(kMagic, kMagic);
+  const float2 half = make_float2(0.5f, 0.5f), magic = make_float2(kMagic, kMagic);
+  // (one by one: the compiler makes one fused instruction of a product of pairs and the sum behind it, and a product next to one half, one in a billion of normal values,
+  // is then not rounded before the sum is)
+  auto scaled = [&](float a, float b) { return make_float2(__fmul_rn(a, scale), __fmul_rn(b, scale)); };
   float most = 0.f;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const float2 y01 = __fadd2_rn(__fmul2_rn(make_float2(v[i].x, v[i].y), s2), half), y23 = __fadd2_rn(__fmul2_rn(make_float2(v[i].z, v[i].w), s2), half);
+    const float2 y01 = __fadd2_rn(scaled(v[i].x, v[i].y), half), y23 = __fadd2_rn(scaled(v[i].z, v[i].w), half);
     most = max3_abs_nan(max3_abs_nan(most, y01.x, y01.y), y23.x, y23.y);
     const float2 n01 = __fadd2_rd(y01, magic), n23 = __fadd2_rd(y23, magic);
     words[i] = __byte_perm(__byte_perm(__float_as_uint(n01.x), __float_as_uint(n01.y), 0x0040),
