@@ -179,6 +179,12 @@ rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
   };
 
   bool ok = true;
+  unsigned waited = FMHA_I8_DEV_WAIT_K_LOAD;         // what for, if not ok
+  auto arrived = [&](bool v) {                       // V has, for all lanes
+    ok = __all_sync(0xFFFFFFFFu, v);
+    if (!ok) waited = FMHA_I8_DEV_WAIT_V_LOAD;
+    return ok;
+  };
   uint32_t n = 0;
   int page = 0, next_page = 0;
   if (first + warp < last) {
@@ -344,7 +350,7 @@ rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
       }
     };
     if constexpr (kRows == 4) {
-      if (!(ok = __all_sync(0xFFFFFFFFu, here))) break;
+      if (!arrived(here)) break;
       products(pa);
     } else if constexpr (kRows == 8) {
       // Are 16 bits enough?  Not where few keys of the tile have most of a row's weight and the others so little that 2^-17 for each counts: where e, none counted with more
@@ -354,7 +360,7 @@ rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
       int all = static_cast<int>((mine & 0xFFFFu) + (mine >> 16));
       bool thin = false;
       if (!__all_sync(0xFFFFFFFFu, here && 4 * all >= least_sum)) {
-        if (!(ok = __all_sync(0xFFFFFFFFu, here))) break;
+        if (!arrived(here)) break;
         all += __shfl_xor_sync(0xFFFFFFFFu, all, 1);
         all += __shfl_xor_sync(0xFFFFFFFFu, all, 2);
         thin = __any_sync(0xFFFFFFFFu, all < least_sum);
@@ -368,6 +374,7 @@ rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
         products(pa);
       }
     } else {
+      if (!arrived(here)) break;
       // sixteen keys at a time
 #pragma unroll
       for (int kb = 0; kb < 8; ++kb) {
@@ -396,7 +403,7 @@ rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
   if (!ok) {
     if (lane == 0) {
       *abort_flag = 1;
-      report(p.status, p.host_word, FMHA_I8_DEV_WAIT_K_LOAD, warp, n);
+      report(p.status, p.host_word, waited, warp, n);
       const long long t0 = clock64();
       while (clock64() - t0 < 2000000LL) { /* copies still in flight land before their memory is used again */ }
     }
