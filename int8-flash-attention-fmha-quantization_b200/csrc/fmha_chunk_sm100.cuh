@@ -582,6 +582,10 @@ template <int D, bool kWide, bool kSplit> __device__ __forceinline__ void softma
 #pragma unroll
           for (int x = 0; x < 32; ++x) o[x] = 0u;
         }
+        if (p.out_down != 1.f) {
+#pragma unroll
+          for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * p.out_down);
+        }
         store32(p.o, p.o_type, p.o_wide != 0, at + i, o, scale);
       }
       __syncwarp();
@@ -642,7 +646,7 @@ template <int D> __device__ __forceinline__ void join_parts(const Params& p, Ctl
       }
       const float scale = l > 0.f ? p.out_scale / l : 0.f;
 #pragma unroll
-      for (int y = 0; y < 4; ++y) a[y] *= scale;
+      for (int y = 0; y < 4; ++y) a[y] = a[y] * scale * p.out_down;
       store4(p.o, p.o_type, (u.seq.q0 + token) * p.o_stride + static_cast<long long>(u.head * p.G + in_tile - my_token * p.G) * D + 4 * c, a);
     }
   }

@@ -46,7 +46,7 @@ struct Params {
   long long first_unit;                // chunk kernel, units not split: those before this one are another launch's
   float c2;                            // from a difference of scores to an exponent of 2
   int growth;                          // chunk kernel: a reference is kept while the maximum exceeds it by no more than this, 2^kGrowth in p
-  float out_scale;                     // from sum p v / sum p, v in codes, to the output's unit
+  float out_scale, out_down;           // from sum p v / sum p, v in codes, to the output's unit: their product (where it is tiny, out_scale over a sum would be none of fp32)
   unsigned* status;                    // eight device status words
   unsigned* host_word;                 // the host-visible failure word
 };

@@ -433,7 +433,7 @@ rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
     if (row >= n_rows) return;
     const float scale = l > 0.f ? p.out_scale / (kWhole ? l * kLevels : l) : 0.f;
 #pragma unroll
-    for (int y = 0; y < 4; ++y) a[y] *= scale;
+    for (int y = 0; y < 4; ++y) a[y] = a[y] * scale * p.out_down;
     store4(p.o, p.o_type, (s.q0 + token) * p.o_stride + static_cast<long long>(head * p.G + row - token * p.G) * D + 4 * c, a);
   };
   float* together = reinterpret_cast<float*>(sm.ring + C::kTileBytes);      // behind the first warp's rows

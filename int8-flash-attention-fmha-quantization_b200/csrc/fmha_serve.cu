@@ -176,7 +176,9 @@ int fill_call(Call* c, const float amax[5], const int desc6[6], const void* q, c
   // between factors at which all probabilities are 1 and at which only the largest counts (the scores are integers up to 2^21)
   p.c2 = static_cast<float>(std::min(std::max(c2, 0x1p-100), 32.0));
   p.growth = static_cast<int>(std::min(static_cast<double>(grouped::kGrowth) / p.c2, 1e9));
-  p.out_scale = o_type == FMHA_I8_TYPE_I8 ? static_cast<float>(static_cast<double>(amax[2]) / amax[3]) : amax[2] / 127.f;
+  const double unit = amax[2] / (o_type == FMHA_I8_TYPE_I8 ? static_cast<double>(amax[3]) : 127.0);
+  p.out_down = unit < 0x1p-60 ? 0x1p-64f : 1.f;
+  p.out_scale = static_cast<float>(unit / p.out_down);
   if (!std::isfinite(p.out_scale)) return FMHA_I8_ERR_BAD_AMAX;
   p.q = static_cast<const int8_t*>(q);
   p.o = o;

@@ -170,3 +170,21 @@ def test_prompts_whose_largest_scores_come_late(pkg, torch, D):
             k[:, :, i] = (levels // 32 + (i < levels % 32).long()).clamp(max=127).to(torch.int8)[:, None]
         for most in (1, 1500):
             bounded(torch, paged(pkg, torch, q, k, v, "bf16", most), q, k, v, "bf16", 1500 / 4, f"{nats} nats every {gap} keys")
+
+
+@pytest.mark.parametrize("D,H,tokens", [(128, 3, 1), (64, 7, 1), (64, 16, 1), (128, 8, 20)])
+def test_tiny_ranges_of_values_and_many_keys(pkg, torch, D, H, tokens):
+    """v_amax = 1e-35: the factor from sums to outputs, v_amax / 127 over a sum of 131,072 keys in units of P, must not fall below what fp32 holds."""
+    keys, page = 131072, 64
+    q, k, v = peaked(torch, tokens, keys, H, 1, D, 0.0, [], 0.3, 60, seed=H)
+    kc, vc = (x.view(keys // page, page, 1, D).transpose(1, 2).contiguous() for x in (k, v))
+    o = torch.empty((tokens, H, D), dtype=torch.bfloat16, device="cuda")
+    for v_amax in (1e-35, 1e35):
+        pkg.FMHAInferI8Paged(None, pkg.FMHAParamI8(AMAX[0], AMAX[1], v_amax, 1.0, 1.0), pkg.AttnDataDescriptorGrouped(1, tokens, keys, H, 1, D), q, kc, vc,
+                             torch.arange(keys // page, dtype=torch.int32, device="cuda")[None], torch.tensor([keys], dtype=torch.int32, device="cuda"), starts([tokens]), o)
+        s = q.double().transpose(0, 1) @ k[:, 0].double().T * scale_of(D)
+        seen = torch.ones((tokens, keys), dtype=torch.bool, device="cuda").tril(keys - tokens)
+        want = (torch.softmax(s.masked_fill(~seen, -math.inf), -1) @ v[:, 0].double()).transpose(0, 1) * (float(torch.tensor(v_amax)) / 127.0)
+        # all values are positive: half a step of the output, and what bounded() counts for P, exp2 and the sums, all relative
+        worst = float(((o.double() - want).abs() / want).max())
+        assert worst <= 2.0 ** -8 + 2.0 ** -11 + 2.0 ** -17 + keys / 4 * 2.0 ** -23, (v_amax, worst)
