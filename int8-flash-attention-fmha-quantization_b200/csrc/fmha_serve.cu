@@ -165,7 +165,7 @@ int fill_call(Call* c, const float amax[5], const int desc6[6], const void* q, c
   if (o_type != FMHA_I8_TYPE_I8 && o_type != FMHA_I8_TYPE_BF16 && o_type != FMHA_I8_TYPE_FP16) return FMHA_I8_ERR_BAD_SHAPE;
   if (total_q < 0 || q_stride < static_cast<long long>(H) * D || o_stride < static_cast<long long>(H) * D) return FMHA_I8_ERR_BAD_SHAPE;
   const int G = H / Hkv;
-  if (total_q > kMostRows / H || static_cast<long long>(max_q) * G > kMostRows - 256 || max_k > (1 << 30) || static_cast<long long>(B) * Hkv > kMostRows) return FMHA_I8_ERR_TOO_LARGE;
+  if (total_q > kMostRows / H || static_cast<long long>(max_q) * G > kMostRows - 256 || max_k > (1 << 30) || B > (1 << 30) || static_cast<long long>(B) * Hkv > kMostRows) return FMHA_I8_ERR_TOO_LARGE;
   if (too_far(total_q, q_stride, 1) || too_far(total_q, o_stride, type_bytes(o_type))) return FMHA_I8_ERR_TOO_LARGE;
   if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(o, 16) || !aligned(cu_q, 4)) return FMHA_I8_ERR_MISALIGNED;
   if (q_stride % 16 != 0 || o_stride * type_bytes(o_type) % 16 != 0) return FMHA_I8_ERR_MISALIGNED;
