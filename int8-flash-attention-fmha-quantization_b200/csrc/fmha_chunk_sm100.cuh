@@ -20,8 +20,8 @@
 // exponentials and their conversion (in halves, P.V of the first beside the second), 770 for P.V and the next scores.  The tiles run half a step apart, so that one's
 // exponentials hide the other's products; a third would need tensor memory that there is not.  A unit's end takes 3700 cycles: the output is read, scaled and stored while the tensor
 // cores have only the other tile.  Tensor pipe 45 % of the cycles, issue 45 %, HBM 9 %.
-//   1 x 16384 tokens, 32 heads on 8 of 128, causal, some values eight times as large   1765 us, 1.25 PFLOP/s (1.35 without those values: references that move)
-//   8 x 2048 tokens                                                                     247 us, 1.11 PFLOP/s; among other calls, at the power limit, 1800 and 267
+//   1 x 16384 tokens, 32 heads on 8 of 128, causal, some values eight times as large   1767 us, 1.25 PFLOP/s (1.34 without those values: references that move)
+//   8 x 2048 tokens                                                                     247 us, 1.11 PFLOP/s; among other calls, at the power limit, 1840 and 266
 #pragma once
 #include "fmha_grouped_sm100.cuh"
 

@@ -8,8 +8,8 @@
 // plane.  With normal values and ranges of 3 to 5 that is one thread in 600 to 1100 where they are rotated, and one in 30 to 120 where bf16 values are not: their products
 // with the scale reach exact halves.
 //
-// 8192 tokens of 48 heads of 128, bf16: 42 us, 3.7 TB/s, 57 % of a copy's rate.  Issue bounds it (57 % of the cycles, 245 instructions of a warp for 512 elements, 4.3 warps
-// to a scheduler): pairs of values in one instruction, the next head's loads ahead and the search of the one pair made 76 us 42.  A range of v whose halves are not reached
+// 8192 tokens of 48 heads of 128, bf16: 42 us, 3.7 TB/s, 57 % of a copy's rate (neighbouring pairs 41, fp16 40, fp32 49).  No unit is full: issue 58 % of the cycles, 245
+// instructions of a warp for 512 elements, DRAM 37 %; 4.4 warps to a scheduler, with one head's loads ahead each, do not hide them all.  Pairs of values in one instruction, the next head's loads ahead and the search of the one pair made 76 us 42.  A range of v whose halves are not reached
 // (3.93 for 4.25) takes 40.6; the division 127 / range taken out of the 64-bit path changes nothing.
 #pragma once
 #include "fmha_grouped_sm100.cuh"

@@ -11,7 +11,7 @@
 //     nothing is converted, no row is idle, and the products of a tile are exact.  It is 65535 e with e relative to the largest score of the tile.
 //     Up to four rows have four bytes each: 65535 e rounded down, and as many bits of what that leaves.  Up to eight have two, rn(65535 e), off by 2^-17 of the
 //     tile's largest e for every key however small its own is; where that may count, in a tile in which few keys have most of a row's weight, they have four too and
-//     there are two products.  (With 16 bits relative to the running maximum 131,072 keys behind one that lies 12.5 nats above them lost a third of their weight.);
+//     there are two products (1190 instructions a tile of four rows, 1280 of eight with one).  (With 16 bits relative to the running maximum 131,072 keys behind one that lies 12.5 nats above them lost a third of their weight.);
 //   * up to sixteen rows P is fp16, 2^15 where p is 1, and V becomes fp16 in registers (integers up to 2048 are exact there), m16n8k16;
 //   * which key, column or row a lane's element belongs to is free as long as both operands agree, and is chosen so that each lane reads 16 bytes at a time
 //     without bank conflicts from the swizzled tiles, and so that the scores' registers are P's operand as they are;
@@ -19,8 +19,8 @@
 //
 // 64 sequences of 1 to 8192 keys, 32 heads on 8 of 128: 105 us, 5.8 TB/s, 88 % of a copy's rate; 172 with P as fp16 (issue: 53 M instructions of six warps to an SM).  64 heads, eight
 // rows: 108, and 117 with two products in every tile.
-// One sequence of 1025 keys: 7.9 us, latencies in a row.  Two of 125,000 keys on 4 key heads, seven rows: 64 us on the 64 SMs that eight clusters
-// of eight have, 3.9 TB/s; 76 with scores of a deviation of 3, most of whose tiles need two products.
+// One sequence of 1025 keys: 7.2 us, latencies in a row.  Two of 125,000 keys on 4 key heads, seven rows: 64 us on the 64 SMs that eight clusters
+// of eight have, 3.9 TB/s; 77 with scores of a deviation of 3, most of whose tiles need two products.
 #pragma once
 #include "fmha_grouped_sm100.cuh"
 

@@ -207,7 +207,7 @@ template <int D, int kRows> int launch_rows(cudaStream_t stream, const Device& d
   const long long n_tiles = (c.max_k + grouped::kTile - 1) / grouped::kTile;
   if (units > kMostRows / rows::kMaxCluster) return FMHA_I8_ERR_TOO_LARGE;      // (B * Hkv is below 2^31, and the groups below 2^29)
   const long long resident = 3LL * dev.sm_count;
-  // Few units with many keys: one CTA with all the warps of an SM on as many SMs as a cluster allows.  8 units of 131,072 keys, head_dim 128: 63 us; the CTAs of
+  // Few units with many keys: one CTA with all the warps of an SM on as many SMs as a cluster allows.  8 units of 131,072 keys, head_dim 128: 64 us; the CTAs of
   // two warps below in clusters of 8 74, of 16 67 to 76.
   const int clusters16 = D == 128 ? g_once[dev.index].clusters16_d128 : g_once[dev.index].clusters16_d64;
   for (const int ctas : {16, 8})
@@ -226,7 +226,7 @@ long long chunk_units(const grouped::Params& p) { return std::min<long long>(p.t
 // Which kernel.  Up to 128 heads share a key head of the chunk kernel, whose tile holds at least one token.  Otherwise by the rows of a sequence and key head
 // (rows kernel against chunk kernel, us): 16 rows, head_dim 128, 4097 keys: 8 units 15.6 and 17.8, 128 units 53 and 60, 512 units 119 and 223.
 // 17 to 32 rows are two groups of the rows kernel, each of which reads all keys: head_dim 64, 129 to 4097 keys, 8 to 1024 units: 0.47 to 0.87 of the chunk
-// kernel's time (512 units of 1025 keys 38 and 62); head_dim 128 0.78 to 0.93 of it for 512 units and more of 1025 keys and more (4097 keys 174 and 223),
+// kernel's time (512 units of 1025 keys 38 and 62); head_dim 128 0.78 to 0.93 of it for 512 units and more of 1025 keys and more (4097 keys 176 and 223),
 // 1.02 to 1.54 for fewer or shorter ones.  33 to 48 rows: 0.60 to 1.08 and 1.05 to 1.22.
 constexpr int kMostGroup = 128;
 bool few_rows(const Call& c, int sms) {
@@ -238,7 +238,7 @@ bool few_rows(const Call& c, int sms) {
 }
 
 // CTAs that share a unit of the chunk kernel, in steps of one key tile (1.7 us): a CTA's share of them, and 4 for what a part costs besides.  Without and with, us:
-// 200 tokens on 32,768 keys (B1 H32/8 D128) 469 and 138, two chunks of 103 on 88,000 (H24/12 D64) 1155 and 317, 16 on 4097 (B1 H32/8 D128) 57 and 20.
+// 200 tokens on 32,768 keys (B1 H32/8 D128) 469 and 147, two chunks of 103 on 88,000 (H24/12 D64) 1155 and 319, 16 on 4097 (B1 H32/8 D128) 57 and 29.
 struct Split { int parts; long long steps; };
 Split chunk_split(long long units, long long n_tiles, int sms) {
   Split best{1, (units + sms - 1) / sms * (n_tiles + 2)};
@@ -255,7 +255,7 @@ long long expected_units(const grouped::Params& p) {
 // The rows of sequences that the rows kernel takes out of a batch of chunks, or 0.  The host does not know the lengths, but the tokens that there are in all: below a quarter of
 // what the sequences may bring.  Steps of the chunk kernel with all sequences against those with the expected ones, 8 for two more launches and the rows kernel's tiles, of
 // which 300 take a step.  In one launch and apart, us (H32/8 D128 where not said): one chunk of 512 among 64 sequences of up to 4096 keys 177 and 118, two of 1024 among 256 of up
-// to 8192 1016 and 596, two of 2048 among 130 288 and 202, one of 480 among 33 of up to 4096 (H16/2 D64) 60 and 52; left in one launch: one of 500 among 5 of up to 1000 20 and 39, 15 of
+// to 8192 1016 and 596, two of 2048 among 130 288 and 202, one of 480 among 33 of up to 4096 (H16/2 D64) 60 and 48; left in one launch: one of 500 among 5 of up to 1000 20 and 39, 15 of
 // 256 among 64 (H12/1) 56 and 71, 8 of 300 among 33 85 and 83.
 int rows_apart(const Call& c, int sms) {
   const grouped::Params& p = c.p;
