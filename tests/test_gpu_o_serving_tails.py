@@ -188,3 +188,15 @@ def test_tiny_ranges_of_values_and_many_keys(pkg, torch, D, H, tokens):
         # all values are positive: half a step of the output, and what bounded() counts for P, exp2 and the sums, all relative
         worst = float(((o.double() - want).abs() / want).max())
         assert worst <= 2.0 ** -8 + 2.0 ** -11 + 2.0 ** -17 + keys / 4 * 2.0 ** -23, (v_amax, worst)
+
+
+@pytest.mark.parametrize("D,H,Hkv,tokens", [(128, 4, 1, 1), (64, 1, 1, 3), (128, 8, 1, 1), (64, 7, 1, 1), (64, 16, 1, 1), (128, 4, 2, 50), (64, 8, 1, 300)])
+def test_the_lowest_code(pkg, torch, D, H, Hkv, tokens):
+    """-128, which the quantiser never gives, in q, k and v at once: largest scores, and the largest sums of bytes that a tile can have."""
+    keys = 1000
+    for q_code, v_code in ((-128, -128), (127, -128), (-128, 127)):
+        q = torch.full((tokens, H, D), q_code, dtype=torch.int8, device="cuda")
+        k = torch.full((keys, Hkv, D), -128, dtype=torch.int8, device="cuda")
+        v = torch.full((keys, Hkv, D), v_code, dtype=torch.int8, device="cuda")
+        o = paged(pkg, torch, q, k, v, "fp16", keys)
+        bounded(torch, o, q, k, v, "fp16", keys / 4, f"{q_code}, {v_code}")
